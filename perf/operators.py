@@ -1,0 +1,428 @@
+"""Operators of cached generation with drafted tokens and a bounded cache, as measurable cases.
+
+``listed()`` holds fixed cases, ``draw(rng)`` one more of the same ranges,
+``prepare(case, seed)`` what a generation loop has in hand before a call,
+``run(state)`` one call (where ``own`` is false the operator's plain form in
+elementary operations, where it is true the framework's entry point),
+``work(case)`` the bytes and operations the call cannot do without and
+``exact(case, seed)`` the result in 64 bits.
+
+Kinds of case (KV caches are [B, Hkv, capacity, D], lengths int32 [B]):
+
+* ``tree``     the drafted tokens of a tree attend the cached prefix and their
+  own ancestors; their keys and values are the last rows of the cache;
+* ``weights``  the attention that the last queries paid to every cached key is
+  added to the keys' weights;
+* ``evict``    the cache is cut to the rows of largest weight, in order;
+* ``accept``   the accepted path of a tree moves to the end of the prefix.
+"""
+
+from __future__ import annotations
+
+import math
+import random
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+SSA_N, SSA_B = 1.5, 0.8  # the framework's initial n and b
+
+
+def _framework():
+    root = str(Path(__file__).resolve().parent.parent / "luciole-1b_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    import SSA
+
+    return SSA
+
+
+def _case(name, kind, **sizes):
+    case = {"kind": kind, **sizes}
+    return dict(case, name=name) if name else case
+
+
+def _tree(name, batch, heads, kv_heads, capacity, dim, nodes, dtype="bf16", own_masks=False):
+    return _case(name, "tree", batch=batch, heads=heads, kv_heads=kv_heads, capacity=capacity, dim=dim, nodes=nodes,
+                 dtype=dtype, own_masks=own_masks)
+
+
+def _weights(name, batch, heads, kv_heads, capacity, dim, queries, dtype="bf16"):
+    return _case(name, "weights", batch=batch, heads=heads, kv_heads=kv_heads, capacity=capacity, dim=dim,
+                 queries=queries, dtype=dtype)
+
+
+def _evict(name, batch, kv_heads, capacity, dim, keep, sinks, recent, dtype="bf16"):
+    return _case(name, "evict", batch=batch, kv_heads=kv_heads, capacity=capacity, dim=dim, keep=keep, sinks=sinks,
+                 recent=recent, dtype=dtype)
+
+
+def _accept(name, batch, kv_heads, capacity, dim, nodes, depth, dtype="bf16"):
+    return _case(name, "accept", batch=batch, kv_heads=kv_heads, capacity=capacity, dim=dim, nodes=nodes, depth=depth,
+                 dtype=dtype)
+
+
+def listed():
+    return [
+        # A lone sequence with a small draft at the 1B decoder's heads: latency.
+        _tree("tree_b1_t8", 1, 16, 16, 2048, 128, 8),
+        # Luciole-1B heads (32 over 8), a serving batch, a usual tree.
+        _tree("tree_gqa_b8_t32", 8, 32, 8, 4096, 64, 32, own_masks=True),
+        # A long document, one sequence, a large tree over grouped heads.
+        _tree("tree_long_t64", 1, 32, 8, 65536, 64, 64),
+        # The benchmark's decode batch with a large tree, in fp16.
+        _tree("tree_b16_t64_fp16", 16, 16, 16, 4096, 128, 64, dtype="fp16"),
+        # Odd sizes: three heads a group, 61 nodes, 1000 rows, head dim 32.
+        _tree("tree_odd_t61", 2, 24, 8, 1000, 32, 61, own_masks=True),
+        # Weights kept up with every generated token of a serving batch.
+        _weights("weights_step_b16", 16, 32, 8, 4096, 64, 1),
+        # The last 32 tokens of a prompt vote on its keys.
+        _weights("weights_window_t32", 4, 16, 16, 8192, 128, 32),
+        # Every token of a prompt votes: Luciole-1B heads, 4096 tokens.
+        _weights("weights_prompt_4096", 1, 32, 8, 4096, 64, 4096),
+        # A serving batch's caches cut to half.
+        _evict("evict_b8", 8, 8, 4096, 64, 2048, 4, 256),
+        # A long prompt cut to a small cache.
+        _evict("evict_long", 1, 16, 32768, 128, 4096, 16, 1024),
+        # A lone sequence accepts a few tokens: latency.
+        _accept("accept_b1", 1, 16, 2048, 128, 8, 4),
+        # A large batch accepts paths of different lengths.
+        _accept("accept_b64", 64, 8, 2048, 64, 64, 16),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+HEADS = [(4, 4), (8, 8), (16, 16), (16, 4), (24, 8), (32, 8), (16, 1)]
+
+
+def draw(rng: random.Random):
+    """One more case of the listed ones' ranges, odd sizes among them."""
+    kind = rng.choices(["tree", "weights", "evict", "accept"], [4, 3, 2, 2])[0]
+    heads, kv_heads = rng.choice(HEADS)
+    dim = rng.choice([32, 64, 64, 128, 128])
+    dtype = rng.choice(["bf16", "bf16", "bf16", "fp16"])
+    batch = _log_int(rng, 1, 16)
+    if kind == "tree":
+        while True:
+            batch, capacity, nodes = _log_int(rng, 1, 16), _log_int(rng, 256, 65536), _log_int(rng, 1, 128)
+            if (batch * heads * nodes * capacity <= 1.3e8 and batch * kv_heads * capacity * dim <= 1.3e8
+                    and nodes <= capacity // 2):
+                return _tree(None, batch, heads, kv_heads, capacity, dim, nodes, dtype, rng.random() < 0.5)
+    if kind == "weights":
+        while True:
+            batch, capacity = _log_int(rng, 1, 16), _log_int(rng, 256, 32768)
+            queries = rng.choice([1, _log_int(rng, 1, 64), _log_int(rng, 1, 4096)])
+            if (batch * heads * queries * capacity <= 5e8 and batch * kv_heads * capacity * dim <= 1.3e8
+                    and queries <= capacity):
+                return _weights(None, batch, heads, kv_heads, capacity, dim, queries, dtype)
+    if kind == "evict":
+        while True:
+            batch, capacity = _log_int(rng, 1, 16), _log_int(rng, 256, 65536)
+            if batch * kv_heads * capacity * dim <= 1.3e8:
+                break
+        keep = max(32, int(capacity * rng.uniform(0.1, 0.9)))
+        return _evict(None, batch, kv_heads, capacity, dim, keep, rng.choice([0, 1, 4, 16]),
+                      rng.randint(0, keep - 16), dtype)
+    nodes = _log_int(rng, 2, 128)
+    return _accept(None, _log_int(rng, 1, 64), kv_heads, rng.choice([1024, 1500, 2048]), dim, nodes,
+                   rng.randint(1, min(nodes, 32)), dtype)
+
+
+def _lengths(case):
+    """Cached tokens of each sequence, fixed by the case: from half the capacity
+    up to all of it (a lone sequence fills it); a prompt's keys are its own."""
+    b, cap = case["batch"], case["capacity"]
+    if b == 1:
+        return [cap]
+    least = max(cap // 2, case.get("queries", 1), case.get("nodes", 1))
+    return [least + (cap - least) * i // (b - 1) for i in range(b)]
+
+
+def _parents(nodes, rng):
+    """A drafted tree: most nodes continue one of the last few, as the beams of a draft do."""
+    return [-1 if i == 0 else max(-1, i - rng.randint(1, 8)) for i in range(nodes)]
+
+
+def _masks(case, seed):
+    """mask[i, j]: node j is node i or one of its ancestors."""
+    rng = random.Random(seed)
+    T, masks = case["nodes"], []
+    for _ in range(case["batch"] if case["own_masks"] else 1):
+        m = torch.zeros(T, T, dtype=torch.bool)
+        for i, p in enumerate(_parents(T, rng)):
+            if p >= 0:
+                m[i] = m[p]
+            m[i, i] = True
+        masks.append(m)
+    return torch.stack(masks) if case["own_masks"] else masks[0]
+
+
+def _caches(case, seed):
+    """Keys and values; a value correlates with its key, as both come from one hidden state."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    shape = (case["batch"], case["kv_heads"], case["capacity"], case["dim"])
+    k = torch.randn(shape, generator=g, device="cuda")
+    v = torch.randn(shape, generator=g, device="cuda").mul_(0.9).add_(k, alpha=0.4)
+    return k.to(DTYPES[case["dtype"]]), v.to(DTYPES[case["dtype"]]), g
+
+
+def _queries(case, rows, g):
+    q = torch.randn(case["batch"], case["heads"], rows, case["dim"], generator=g, device="cuda")
+    return q.to(DTYPES[case["dtype"]])
+
+
+def _int32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _normalisers(case, q, k, lens):
+    """m of every query, as the attention that ran before left it."""
+    T, G, D = case["queries"], case["heads"] // case["kv_heads"], case["dim"]
+    m = torch.empty(q.shape[:3], device="cuda")
+    for b, L in enumerate(lens):
+        seen = torch.arange(L, device="cuda")[None, :] <= torch.arange(L - T, L, device="cuda")[:, None]
+        for h in range(case["heads"]):
+            s = (q[b, h].float() @ k[b, h // G, :L].float().t()) / math.sqrt(D)
+            t = SSA_N * s.sign() * torch.log1p(SSA_B * s.abs())
+            m[b, h] = t.masked_fill_(~seen, -math.inf).logsumexp(-1) / math.log(2.0)
+    return m
+
+
+def _key_weights(case, g):
+    """Accumulated weights as attention leaves them: a few large, most small."""
+    shape = (case["batch"], case["kv_heads"], case["capacity"])
+    return torch.randn(shape, generator=g, device="cuda").mul_(1.5).exp_()
+
+
+def _paths(case, seed):
+    """Accepted nodes of each sequence, in ascending order, and how many they are."""
+    rng = random.Random(seed)
+    paths = [sorted(rng.sample(range(case["nodes"]), case["depth"])) for _ in range(case["batch"])]
+    return paths, [rng.randint(1, case["depth"]) for _ in range(case["batch"])]
+
+
+def prepare(case, seed):
+    kind, lens = case["kind"], _lengths(case)
+    k, v, g = _caches(case, seed)
+    state = {"case": case, "k": k, "v": v, "lens": _int32(lens)}
+    if kind in ("tree", "weights"):
+        state.update(scale=1.0 / math.sqrt(case["dim"]), n=torch.tensor(SSA_N, device="cuda"),
+                     b=torch.tensor(SSA_B, device="cuda"))
+    if kind == "tree":
+        state.update(q=_queries(case, case["nodes"], g), mask=_masks(case, seed).cuda())
+    elif kind == "weights":
+        q = _queries(case, case["queries"], g)
+        state.update(q=q, m=_normalisers(case, q, k, lens), weights=_key_weights(case, g))
+    elif kind == "evict":
+        state.update(weights=_key_weights(case, g))
+    else:
+        paths, counts = _paths(case, seed)
+        state.update(path=_int32(paths), accepted=_int32(counts))
+    return state
+
+
+def _scores(state):
+    """t = n sign(s) ln(1 + b |s|) of every query row [B, Hkv, G, T, capacity]."""
+    q, k = state["q"].float(), state["k"].float()
+    B, H, T, D = q.shape
+    Hk, cap = k.shape[1], k.shape[2]
+    s = state["scale"] * (q.view(B, Hk, H // Hk * T, D) @ k.transpose(2, 3)).view(B, Hk, H // Hk, T, cap)
+    return state["n"] * s.sign() * torch.log1p(state["b"] * s.abs())
+
+
+def _first(state, queries):
+    """Position of the first of the last `queries` rows of each sequence [B, 1, 1]."""
+    return (state["lens"].long() - queries)[:, None, None]
+
+
+def _plain_tree(state):
+    T, cap = state["q"].shape[2], state["k"].shape[2]
+    first = _first(state, T)
+    at = torch.arange(cap, device="cuda")[None, None, :]
+    node = (at - first).expand(-1, T, -1)
+    mask = state["mask"].expand(node.shape[0], T, T)
+    seen = (node < 0) | ((node < T) & mask.gather(2, node.clamp(0, T - 1)))
+    t = _scores(state).masked_fill(~seen[:, None, None], -math.inf)
+    top = t.amax(-1, keepdim=True)
+    p = (t - top).exp()
+    total = p.sum(-1, keepdim=True)
+    B, Hk, G = t.shape[:3]
+    o = (p / total).view(B, Hk, G * T, cap) @ state["v"].float()
+    m = ((top + total.log()) / math.log(2.0)).view(B, Hk * G, T)
+    return {"out": o.view(B, Hk * G, T, -1).to(state["q"].dtype), "m": m}
+
+
+def _plain_weights(state):
+    T, cap = state["q"].shape[2], state["k"].shape[2]
+    B, Hk = state["k"].shape[:2]
+    at = torch.arange(cap, device="cuda")
+    seen = at[None, None, :] <= _first(state, T) + torch.arange(T, device="cuda")[None, :, None]
+    m = state["m"].view(B, Hk, -1, T, 1)
+    p = (_scores(state) - m * math.log(2.0)).exp().masked_fill(~seen[:, None, None], 0.0)
+    state["weights"] += p.sum((2, 3))
+    return {"weights": state["weights"]}
+
+
+def _plain_evict(state):
+    case, w, lens = state["case"], state["weights"], state["lens"].long()
+    keep, cap = case["keep"], case["capacity"]
+    B, Hk = w.shape[:2]
+    at = torch.arange(cap, device="cuda")
+    L = lens[:, None, None]
+    must = (at < case["sinks"]) | ((at >= L - case["recent"]) & (at < L))
+    rank = w.masked_fill(must, math.inf).masked_fill((at >= L).expand_as(must).expand_as(w), -math.inf)
+    order = rank.sort(dim=-1, descending=True, stable=True)[1][..., :keep]
+    new = lens.clamp(max=keep)
+    inside = torch.arange(keep, device="cuda") < new[:, None, None]
+    kept = order.masked_fill(~inside, cap).sort(dim=-1)[0]
+    rows = kept.clamp(max=cap - 1)
+    for_rows = rows[..., None].expand(-1, -1, -1, case["dim"])
+    for name in ("k", "v"):
+        c = state[name]
+        c[:, :, :keep] = torch.where(inside[..., None], c.gather(2, for_rows), c[:, :, :keep])
+    left = torch.zeros_like(w)
+    left[..., :keep] = w.gather(2, rows).masked_fill(~inside, 0.0)
+    kept = kept.masked_fill(~inside, -1).int()
+    return {"lens": new.int(), "weights": left, "kept": kept, "k": state["k"], "v": state["v"]}
+
+
+def _plain_accept(state):
+    case, path, count = state["case"], state["path"].long(), state["accepted"].long()
+    first = (state["lens"].long() - case["nodes"])[:, None]
+    step = torch.arange(path.shape[1], device="cuda")[None, :]
+    ok = (step < count[:, None])[..., None, None]
+    b = torch.arange(path.shape[0], device="cuda")[:, None]
+    for name in ("k", "v"):
+        c = state[name]
+        c[b, :, first + step] = torch.where(ok, c[b, :, first + path], c[b, :, first + step])
+    return {"lens": (first[:, 0] + count).int(), "k": state["k"], "v": state["v"]}
+
+
+def _own(state):
+    case, ssa = state["case"], _framework()
+    if case["kind"] == "tree":
+        out, m = ssa.ssa_tree_attention(state["q"], state["k"], state["v"], state["lens"], state["mask"],
+                                        state["scale"], state["n"], state["b"], return_m=True)
+        return {"out": out, "m": m}
+    if case["kind"] == "weights":
+        return {"weights": ssa.ssa_key_weights(state["q"], state["k"], state["m"], state["lens"], state["weights"],
+                                               state["scale"], state["n"], state["b"])}
+    if case["kind"] == "evict":
+        lens, weights, kept = ssa.ssa_cache_evict(state["k"], state["v"], state["lens"], state["weights"],
+                                                  case["keep"], sinks=case["sinks"], recent=case["recent"])
+        return {"lens": lens, "weights": weights, "kept": kept, "k": state["k"], "v": state["v"]}
+    lens = ssa.ssa_cache_accept(state["k"], state["v"], state["lens"], state["path"], state["accepted"],
+                                case["nodes"])
+    return {"lens": lens, "k": state["k"], "v": state["v"]}
+
+
+PLAIN = {"tree": _plain_tree, "weights": _plain_weights, "evict": _plain_evict, "accept": _plain_accept}
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return PLAIN[state["case"]["kind"]](state)
+
+
+def _pairs(case, queries):
+    return case["heads"] * sum(L * queries - queries * (queries - 1) // 2 for L in _lengths(case))
+
+
+def work(case):
+    kind, D, Hk, total = case["kind"], case["dim"], case["kv_heads"], sum(_lengths(case))
+    B = case["batch"]
+    if kind == "tree":
+        # keys and values read, q read, out and m written, the mask read
+        T = case["nodes"]
+        rows = B * case["heads"] * T
+        pairs = case["heads"] * T * (total - B * T)  # the prefix; the tree's own pairs are few
+        return {"bytes": 4 * total * Hk * D + rows * (4 * D + 4) + (B if case["own_masks"] else 1) * T * T,
+                "flops": 4 * D * pairs}
+    if kind == "weights":
+        # keys read, q and m read, weights read and written
+        T = case["queries"]
+        return {"bytes": total * Hk * (2 * D + 8) + B * case["heads"] * T * (2 * D + 4),
+                "flops": 2 * D * _pairs(case, T)}
+    if kind == "evict":
+        # weights read and written, the kept rows of K and V read and written, their places written
+        rows = B * Hk * case["keep"]
+        return {"bytes": 4 * total * Hk + 4 * B * Hk * case["capacity"] + rows * (8 * D + 4), "flops": 0}
+    # from 1 to depth rows move, (depth + 1) / 2 of them on average
+    return {"bytes": B * (case["depth"] + 1) * (4 * Hk * D + 2) + 12 * B, "flops": 0}
+
+
+def _head64(q, k, v, mask, m=None):
+    """One head in 64 bits, rows in pieces: the output and m, or with m the weight of every key."""
+    out, norm = torch.zeros_like(q), torch.empty(q.shape[0], dtype=torch.float64, device=q.device)
+    weight = torch.zeros(k.shape[0], dtype=torch.float64, device=q.device)
+    for i in range(0, q.shape[0], 1024):
+        s = q[i:i + 1024] @ k.t() / math.sqrt(q.shape[1])
+        t = torch.where(s < 0, -SSA_N, SSA_N) * (1 + SSA_B * s.abs()).log()
+        e = torch.where(mask[i:i + 1024], t.exp(), torch.zeros_like(t))
+        if m is not None:
+            weight += (e * torch.exp2(-m[i:i + 1024, None])).sum(0)
+            continue
+        z = e.sum(1, keepdim=True)
+        out[i:i + 1024] = torch.where(z > 0, e @ v / z.clamp_min(1e-300), torch.zeros_like(out[i:i + 1024]))
+        norm[i:i + 1024] = z[:, 0].log2()
+    return out, norm, weight
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    kind, lens, k, v = case["kind"], _lengths(case), state["k"], state["v"]
+    if kind in ("evict", "accept"):
+        return _moved(case, seed, state)
+    G = case["heads"] // case["kv_heads"]
+    q = state["q"]
+    out, m = torch.empty(q.shape, dtype=torch.float64, device="cuda"), None
+    weights = state["weights"].double() if kind == "weights" else None
+    m = torch.empty(q.shape[:3], dtype=torch.float64, device="cuda")
+    T = q.shape[2]
+    for i, L in enumerate(lens):
+        if kind == "tree":
+            own_rows = state["mask"][i] if case["own_masks"] else state["mask"]
+            mask = torch.cat([torch.ones(T, L - T, dtype=torch.bool, device="cuda"), own_rows], 1)
+        else:
+            mask = torch.ones(T, L, dtype=torch.bool, device="cuda").tril(L - T)
+        for h in range(case["heads"]):
+            kh, vh = k[i, h // G, :L].double(), v[i, h // G, :L].double()
+            given = state["m"][i, h].double() if kind == "weights" else None
+            o, norm, w = _head64(q[i, h].double(), kh, vh, mask, given)
+            if kind == "weights":
+                weights[i, h // G, :L] += w
+            else:
+                out[i, h], m[i, h] = o, norm
+    return {"weights": weights} if kind == "weights" else {"out": out, "m": m}
+
+
+def _moved(case, seed, state):
+    """The caches after the rows moved, one sequence and head at a time."""
+    lens = _lengths(case)
+    k, v = state["k"].clone(), state["v"].clone()
+    if case["kind"] == "accept":
+        paths, counts = _paths(case, seed)
+        for i, L in enumerate(lens):
+            for to, at in enumerate(paths[i][:counts[i]]):
+                first = L - case["nodes"]
+                k[i, :, first + to], v[i, :, first + to] = state["k"][i, :, first + at], state["v"][i, :, first + at]
+        return {"lens": None, "k": k.double(), "v": v.double()}
+    w = torch.zeros_like(state["weights"], dtype=torch.float64)
+    for i, L in enumerate(lens):
+        for h in range(case["kv_heads"]):
+            u = state["weights"][i, h, :L].double().clone()
+            u[:case["sinks"]] = math.inf
+            u[max(0, L - case["recent"]):] = math.inf
+            n = min(L, case["keep"])
+            rows = u.argsort(dim=-1, descending=True, stable=True)[:n].sort()[0]
+            k[i, h, :n], v[i, h, :n] = state["k"][i, h, rows], state["v"][i, h, rows]
+            w[i, h, :n] = state["weights"][i, h, rows].double()
+    return {"lens": None, "weights": w, "kept": None, "k": k.double(), "v": v.double()}
