@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define SSA_ABI_VERSION 6
+#define SSA_ABI_VERSION 7
 
 /* Status codes. */
 enum {

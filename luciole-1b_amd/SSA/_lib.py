@@ -54,9 +54,15 @@ EXPORTED_SYMBOLS = (
     "ssa_swiglu",
     "ssa_cross_entropy",
     "ssa_embedding_bwd",
+    "ssa_tree_num_splits",  # include/ssa_cache_ops.h
+    "ssa_tree_workspace_bytes",
+    "ssa_tree_attention",
+    "ssa_key_weights",
+    "ssa_cache_evict",
+    "ssa_cache_accept",
 )
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 
 class Tensor4(ctypes.Structure):
@@ -243,6 +249,101 @@ class DecodeArgs(ctypes.Structure):
     ]
 
 
+class TreeArgs(ctypes.Structure):
+    """ssa_tree_args of include/ssa_cache_ops.h."""
+
+    _fields_ = [
+        ("q", Tensor4),
+        ("k_cache", Tensor4),
+        ("v_cache", Tensor4),
+        ("out", Tensor4),
+        ("m", ctypes.c_void_p),
+        ("cache_seqlens", ctypes.c_void_p),
+        ("tree_mask", ctypes.c_void_p),
+        ("mask_stride_b", ctypes.c_int64),
+        ("ssa_n", ctypes.c_void_p),
+        ("ssa_b", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("heads_q", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("nodes", ctypes.c_int32),
+        ("num_splits", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+    ]
+
+
+class KeyWeightsArgs(ctypes.Structure):
+    """ssa_key_weights_args of include/ssa_cache_ops.h."""
+
+    _fields_ = [
+        ("q", Tensor4),
+        ("k_cache", Tensor4),
+        ("m", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("weights_stride_b", ctypes.c_int64),
+        ("weights_stride_h", ctypes.c_int64),
+        ("cache_seqlens", ctypes.c_void_p),
+        ("ssa_n", ctypes.c_void_p),
+        ("ssa_b", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("heads_q", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("queries", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+    ]
+
+
+class CacheEvictArgs(ctypes.Structure):
+    """ssa_cache_evict_args of include/ssa_cache_ops.h."""
+
+    _fields_ = [
+        ("k_cache", Tensor4),
+        ("v_cache", Tensor4),
+        ("weights", ctypes.c_void_p),
+        ("weights_stride_b", ctypes.c_int64),
+        ("weights_stride_h", ctypes.c_int64),
+        ("cache_seqlens", ctypes.c_void_p),
+        ("seqlens_out", ctypes.c_void_p),
+        ("weights_out", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("keep", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+    ]
+
+
+class CacheAcceptArgs(ctypes.Structure):
+    """ssa_cache_accept_args of include/ssa_cache_ops.h."""
+
+    _fields_ = [
+        ("k_cache", Tensor4),
+        ("v_cache", Tensor4),
+        ("cache_seqlens", ctypes.c_void_p),
+        ("path", ctypes.c_void_p),
+        ("accepted", ctypes.c_void_p),
+        ("seqlens_out", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("nodes", ctypes.c_int32),
+        ("depth", ctypes.c_int32),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -267,7 +368,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     for name, argt in (("ssa_varlen_fwd", VarlenFwdArgs), ("ssa_varlen_bwd", VarlenBwdArgs),
                        ("ssa_decode", DecodeArgs), ("ssa_rope", RopeArgs), ("ssa_rmsnorm_fwd", RmsNormFwdArgs),
                        ("ssa_rmsnorm_bwd", RmsNormBwdArgs), ("ssa_swiglu", SwigluArgs),
-                       ("ssa_cross_entropy", CrossEntropyArgs), ("ssa_embedding_bwd", EmbeddingBwdArgs)):
+                       ("ssa_cross_entropy", CrossEntropyArgs), ("ssa_embedding_bwd", EmbeddingBwdArgs),
+                       ("ssa_tree_attention", TreeArgs), ("ssa_key_weights", KeyWeightsArgs),
+                       ("ssa_cache_evict", CacheEvictArgs), ("ssa_cache_accept", CacheAcceptArgs)):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int32
         fn.argtypes = [ctypes.POINTER(argt), ctypes.c_void_p]
@@ -278,6 +381,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ssa_rmsnorm_workspace_floats.argtypes = [i32, i32]
     lib.ssa_decode_workspace_bytes.restype = ctypes.c_int64
     lib.ssa_decode_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32]
+    lib.ssa_tree_num_splits.restype = ctypes.c_int32
+    lib.ssa_tree_num_splits.argtypes = [i32] * 6
+    lib.ssa_tree_workspace_bytes.restype = ctypes.c_int64
+    lib.ssa_tree_workspace_bytes.argtypes = [i32] * 7
 
 
 def lib() -> ctypes.CDLL:
@@ -302,10 +409,12 @@ def lib() -> ctypes.CDLL:
 
 
 # The launch layer's extension module (csrc/torch_native.cpp), and the C ABI
-# entry points it calls, in the order its bind() takes them.
+# entry points it calls, in the order its bind() and bind_cache() take them.
 NATIVE_PATH = Path(__file__).resolve().parent / "_ssa_native.so"
 _NATIVE_ENTRIES = ("ssa_fwd", "ssa_bwd", "ssa_varlen_fwd", "ssa_varlen_bwd", "ssa_decode", "ssa_bwd_partials_count",
                    "ssa_bwd_ds_workspace_bytes", "ssa_varlen_bwd_ds_workspace_bytes", "ssa_decode_workspace_bytes")
+_NATIVE_CACHE_ENTRIES = ("ssa_tree_attention", "ssa_tree_workspace_bytes", "ssa_key_weights", "ssa_cache_evict",
+                         "ssa_cache_accept")
 _native = None
 
 
@@ -338,7 +447,9 @@ def _open_native(handle):
                           f"{handle.ssa_abi_version()}")
     if not torch.__version__.startswith(mod.TORCH_VERSION):
         raise ImportError(f"{NATIVE_PATH} is built for PyTorch {mod.TORCH_VERSION}, this is {torch.__version__}")
-    mod.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in _NATIVE_ENTRIES))
+    address = lambda name: ctypes.cast(getattr(handle, name), ctypes.c_void_p).value  # noqa: E731
+    mod.bind(*map(address, _NATIVE_ENTRIES))
+    mod.bind_cache(*map(address, _NATIVE_CACHE_ENTRIES))
     return mod
 
 

@@ -1,0 +1,245 @@
+// Rows of a KV cache moved in place: eviction by weight and the acceptance of a
+// drafted path, for gfx950.
+//
+// Eviction keeps `keep` rows of each (sequence, kv-head).  evict_select_kernel
+// finds the weight of the last row that stays by a radix selection over the
+// weights' bits in an order-preserving form (three histograms of 11, 11 and 10
+// bits), then writes the kept rows' indices and weights in ascending order: a
+// row's place is the number of rows before it that stay, that is of rows above
+// the threshold plus the smaller of the rows at it and the number of those that
+// stay, so one scan of two counts places everything.  evict_move_kernel moves
+// the rows.  In place and in order: place i's row comes from kept[i] >= i, and
+// chunk by chunk every source is read before the chunk's places are written;
+// a later chunk's sources lie behind every place written so far.
+#include "ssa_cache_ops.hpp"
+#include "ssa_common.hpp"
+#include "ssa_launch.hpp"
+
+namespace ssa {
+
+namespace {
+
+constexpr int kSelect = 1024;  // threads of a selection
+constexpr int kBins = 2048;
+
+// Unsigned order of weights: NaN below everything, -0 equal to +0.
+__device__ __forceinline__ uint32_t order_bits(float w) {
+  if (w != w) return 0;
+  const uint32_t u = __float_as_uint(w + 0.f);
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ int clamped_len(const int* lens, int b, int cap) {
+  const int L = load_table_entry(lens, b);
+  return L < 0 ? 0 : (L > cap ? cap : L);
+}
+
+// Inclusive sum over the workgroup's threads (kSelect of them); `waves` holds
+// one value per wave.  Two barriers.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* waves, int tid, uint32_t& total) {
+  const int lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t y = __shfl_up(x, off, 64);
+    if (lane >= off) x += y;
+  }
+  __syncthreads();  // the last scan's values have been read
+  if (lane == 63) waves[wave] = x;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kSelect / 64; ++w) {
+    const uint32_t v = waves[w];
+    before += w < wave ? v : 0;
+    all += v;
+  }
+  total = all;
+  return x + before;
+}
+
+}  // namespace
+
+__global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams p, int nblocks) {
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t waves[kSelect / 64];
+  __shared__ uint32_t found[2];  // digit, rows above it
+  const int tid = threadIdx.x, block = folded_block();
+  if (block >= nblocks) return;
+  const int b = block / p.Hkv, h = block - b * p.Hkv;
+  const int L = clamped_len(p.seqlens, b, p.cap);
+  const float* w = p.w + b * p.w_sb + h * p.w_sh;
+  const int64_t bh = block;
+  float* w_out = p.w_out + bh * p.cap;
+  int* kept = p.kept + bh * p.keep;
+  if (h == 0 && tid == 0) p.lens_out[b] = min(L, p.keep);
+  if (L <= p.keep) {
+    for (int i = tid; i < p.cap; i += kSelect) w_out[i] = i < L ? w[i] : 0.f;
+    for (int i = tid; i < p.keep; i += kSelect) kept[i] = i < L ? i : -1;
+    return;
+  }
+  // rows [lo, hi) are chosen from; sinks + recent <= keep < L, so lo < hi
+  const int lo = p.sinks, hi = L - p.recent;
+  uint32_t need = p.keep - p.sinks - p.recent;  // of them stay, fewer than there are
+  uint32_t prefix = 0, ties = 0;
+  const bool choose = need > 0;
+  if (choose) {
+    constexpr int kShift[3] = {21, 10, 0}, kWidth[3] = {11, 11, 10};
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      for (int i = tid; i < kBins; i += kSelect) hist[i] = 0;
+      __syncthreads();
+      const int shift = kShift[pass];
+      const uint32_t mask = (1u << kWidth[pass]) - 1u;
+      for (int i = lo + tid; i < hi; i += kSelect) {
+        const uint32_t key = order_bits(w[i]);
+        if (pass == 0 || (key >> (shift + kWidth[pass])) == prefix) atomicAdd(&hist[(key >> shift) & mask], 1u);
+      }
+      __syncthreads();
+      // bins from the top: thread i takes bins 2047 - 2 i and the one below
+      const uint32_t h0 = hist[kBins - 1 - 2 * tid], h1 = hist[kBins - 2 - 2 * tid];
+      uint32_t total;
+      const uint32_t upto = block_scan(h0 + h1, waves, tid, total);
+      const uint32_t above = upto - h0 - h1;
+      if (above < need && upto >= need) {
+        const bool second = above + h0 < need;
+        found[0] = kBins - 1 - 2 * tid - (second ? 1 : 0);
+        found[1] = second ? above + h0 : above;
+      }
+      __syncthreads();
+      prefix = (prefix << kWidth[pass]) | found[0];
+      need -= found[1];
+    }
+    ties = need;  // rows at the threshold that stay, the lowest first
+  }
+  // places: 4 consecutive rows a thread
+  uint32_t above0 = 0, at0 = 0;  // rows before this stretch that surely stay; at the threshold
+  for (int r0 = 0; r0 < L; r0 += 4 * kSelect) {
+    float v[4];
+    uint32_t up[4], eq[4], count = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = r0 + 4 * tid + e;
+      v[e] = i < L ? w[i] : 0.f;
+      const uint32_t key = order_bits(v[e]);
+      const bool inside = i >= lo && i < hi;
+      up[e] = i < L && (!inside || (choose && key > prefix));
+      eq[e] = inside && choose && key == prefix;
+      count += up[e] + (eq[e] << 16);
+    }
+    uint32_t total;
+    uint32_t before = block_scan(count, waves, tid, total) - count;  // both below 2^13: no carry
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t at = at0 + (before >> 16), place = above0 + (before & 0xffffu) + (at < ties ? at : ties);
+      if (up[e] || (eq[e] && at < ties)) {
+        kept[place] = r0 + 4 * tid + e;
+        w_out[place] = v[e];
+      }
+      before += up[e] + (eq[e] << 16);
+    }
+    above0 += total & 0xffffu;
+    at0 += total >> 16;
+  }
+  for (int i = p.keep + tid; i < p.cap; i += kSelect) w_out[i] = 0.f;
+}
+
+// One workgroup per (tensor, sequence, kv-head, slice of SP 16-byte pieces of a row).
+template <int SP>
+__global__ __launch_bounds__(1024) void evict_move_kernel(EvictParams p, int slices, int nblocks) {
+  constexpr int U = 4, ROWS = 1024 / SP;  // rows of one step, U steps a chunk
+  const int block = folded_block();
+  if (block >= nblocks) return;
+  int u = block;
+  const int slice = u % slices;
+  u /= slices;
+  const Tensor4& t = (u & 1) ? p.v : p.k;
+  u >>= 1;
+  const int h = u % p.Hkv, b = u / p.Hkv;
+  const int L = clamped_len(p.seqlens, b, p.cap);
+  if (L <= p.keep) return;
+  const int* kept = p.kept + static_cast<int64_t>(u) * p.keep;
+  const int tid = threadIdx.x, piece = slice * SP + tid % SP, row = tid / SP;
+  char* base = static_cast<char*>(const_cast<void*>(t.ptr)) + (b * t.sb + h * t.sh) * 2 + piece * 16;
+  for (int r0 = 0; r0 < p.keep; r0 += U * ROWS) {
+    u32x4 v[U];
+    bool moves[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int r = r0 + j * ROWS + row;
+      const int src = r < p.keep ? kept[r] : r;
+      moves[j] = src != r;
+      if (moves[j]) v[j] = *reinterpret_cast<const u32x4*>(base + static_cast<int64_t>(src) * t.ss * 2);
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // the chunk's rows are in registers ...
+    __syncthreads();                // ... everywhere
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int r = r0 + j * ROWS + row;
+      if (moves[j]) *reinterpret_cast<u32x4*>(base + static_cast<int64_t>(r) * t.ss * 2) = v[j];
+    }
+  }
+}
+
+// One workgroup per (tensor, sequence, kv-head, slice of `sp` pieces): all
+// depth * sp <= 1024 pieces are read before the first is written, so the path
+// may be in any order.
+__global__ __launch_bounds__(256) void accept_kernel(AcceptParams p, int sp, int slices, int nblocks) {
+  const int block = folded_block();
+  if (block >= nblocks) return;
+  int u = block;
+  const int slice = u % slices;
+  u /= slices;
+  const bool is_v = u & 1;
+  const Tensor4& t = is_v ? p.v : p.k;
+  u >>= 1;
+  const int h = u % p.Hkv, b = u / p.Hkv;
+  const int L = clamped_len(p.seqlens, b, p.cap);
+  const int first = L - p.T;
+  int n = load_table_entry(p.accepted, b);
+  n = first < 0 ? 0 : (n < 0 ? 0 : (n > p.depth ? p.depth : n));
+  if (threadIdx.x == 0 && slice == 0 && !is_v && h == 0) p.lens_out[b] = first < 0 ? L : first + n;
+  if (n == 0) return;
+  const int pieces = p.D / 8;
+  char* base = static_cast<char*>(const_cast<void*>(t.ptr)) + (b * t.sb + h * t.sh) * 2;
+  u32x4 v[4];
+  int64_t to[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int e = threadIdx.x + 256 * j, i = e / sp, piece = slice * sp + e - i * sp;
+    to[j] = -1;
+    if (i < n && piece < pieces) {
+      int node = p.path[static_cast<int64_t>(b) * p.depth + i];
+      node = node < 0 ? 0 : (node >= p.T ? p.T - 1 : node);
+      if (node != i) {
+        to[j] = (first + i) * t.ss * 2 + piece * 16;
+        v[j] = *reinterpret_cast<const u32x4*>(base + (first + node) * t.ss * 2 + piece * 16);
+      }
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // the rows are in registers ...
+  __syncthreads();                // ... everywhere
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (to[j] >= 0) *reinterpret_cast<u32x4*>(base + to[j]) = v[j];
+}
+
+hipError_t launch_evict(const EvictParams& p, hipStream_t s) {
+  const int heads = p.B * p.Hkv;
+  hipLaunchKernelGGL(evict_select_kernel, folded_grid(heads, kSelect), dim3(kSelect), 0, s, p, heads);
+  const int slices = p.D / 8 / 4;  // 64-byte slices
+  const int blocks = heads * 2 * slices;
+  hipLaunchKernelGGL((evict_move_kernel<4>), folded_grid(blocks, 1024), dim3(1024), 0, s, p, slices, blocks);
+  return hipGetLastError();
+}
+
+hipError_t launch_accept(const AcceptParams& p, hipStream_t s) {
+  const int pieces = p.D / 8;
+  const int most = 1024 / p.depth;  // >= 1: depth <= 1024
+  const int sp = pieces < most ? pieces : most;
+  const int slices = (pieces + sp - 1) / sp;
+  const int blocks = p.B * p.Hkv * 2 * slices;
+  hipLaunchKernelGGL(accept_kernel, folded_grid(blocks, 256), dim3(256), 0, s, p, sp, slices, blocks);
+  return hipGetLastError();
+}
+
+}  // namespace ssa

@@ -1,0 +1,232 @@
+// The attention that query rows paid to cached keys, added to the keys'
+// weights, for gfx950:
+//   w_j += sum over rows r that see key j of p_rj,  p_rj = 2^(t_rj - m_r),
+//   t_rj = n sign(s) log2(1 + scale b |s|),  s = q_r . k_j
+// with the rows' normalisers m given, so one pass over the rows suffices and
+// nothing but the scores' products is needed: S = Q K^T (A = 32 rows of Q from
+// LDS, B = 32 keys in registers), whose result holds one key per lane pair and
+// 16 rows in each lane's registers.  A key's sum over the rows stays in its
+// lanes from the first row to the last (fp32, fixed order, no atomics).
+//
+// The G heads of a group and their T queries are rows r = t * G + head, so the
+// causal mask only bounds the first row of a workgroup's keys and the rows
+// near it.  A workgroup is KW key waves of 32 NK keys by RW row waves of 32
+// rows; Q rows pass through LDS in stages of 32 RW rows, two in flight.
+#include "ssa_cache_ops.hpp"
+#include "ssa_common.hpp"
+#include "ssa_launch.hpp"
+#include "ssa_tile.hpp"
+
+namespace ssa {
+
+namespace {
+
+template <int D, int KW, int RW, int NK>
+struct WeightsCfg {
+  static constexpr int NW = KW * RW;
+  static constexpr int KEYS = 32 * KW * NK;
+  static constexpr int ROWS = 32 * RW;              // rows of a stage
+  static constexpr int QB = ROWS * D * 2;           // bytes of its Q rows
+  static constexpr int PIECES = BlockLayout<D>::IPB;  // 1 KB pieces of a 32-row block
+};
+
+}  // namespace
+
+template <typename T, int D, int KW, int RW, int NK>
+__global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsParams p, int ntiles, int nblocks) {
+  using C = WeightsCfg<D, KW, RW, NK>;
+  typedef typename Vec8<T>::type v8;
+  constexpr int ND16 = D / 16;
+  static_assert(KW % 2 == 0, "one piece parity per wave");
+  __shared__ __attribute__((aligned(1024))) char qs[2 * C::QB];
+  __shared__ __attribute__((aligned(16))) float ms[2][C::ROWS];  // m of the stage's rows
+  __shared__ __attribute__((aligned(16))) int ps[2][C::ROWS];    // and their positions; -1: adds nothing
+  __shared__ int odd[2][RW];  // a row of the block adds nothing
+  __shared__ float part[C::NW][32 * NK];
+
+  const int block = folded_block();
+  if (block >= nblocks) return;
+  // all (sequence, head) pairs of a key tile together: the tiles of most rows come first
+  const int nbh = p.B * p.Hkv;
+  const int tile = block / nbh, bh = block - tile * nbh;
+  const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  int L = load_table_entry(p.seqlens, b);
+  L = L < 0 ? 0 : (L > p.cap ? p.cap : L);
+  const int key0 = tile * C::KEYS;
+  if (key0 >= L) return;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kw = wave / RW, rw = wave - kw * RW;
+  const int l32 = lane & 31, hh = lane >> 5;
+  const int G = p.Hq / p.Hkv, R = G * p.T, first = L - p.T;  // first: position of query 0
+  const float n = *p.n_ptr, c = p.scale * *p.b_ptr;
+  const int kbase = key0 + 32 * NK * kw;  // this wave's keys
+
+  // rows from the first query that sees key0 on
+  const int tstart = key0 > first ? key0 - first : 0;
+  const int rstart = tstart * G;  // < R: key0 < L
+  const int nst = (R - rstart + C::ROWS - 1) / C::ROWS;
+
+  // the row of its block that this lane's loads fetch, as (query, head), moved
+  // on by one stage at a time
+  const LoadLane ll(lane, kw, p.q.ss);
+  int t, g;
+  {
+    const int r = rstart + 32 * rw + ll.r;
+    t = r / G;
+    g = r - t * G;
+  }
+  const int dt = C::ROWS / G, dg = C::ROWS - dt * G;
+  const char* qbase = static_cast<const char*>(p.q.ptr) + (b * p.q.sb + static_cast<int64_t>(hk) * G * p.q.sh) * 2;
+  const float* mbase = p.m + (static_cast<int64_t>(b) * p.Hq + hk * G) * p.T;
+  const uint32_t lds0 = lds_addr(qs);
+  float mv = 0.f;
+  int pv = -1;
+  auto issue = [&](int i) {
+    const bool in = t < p.T;
+    const int tt = in ? t : p.T - 1, gg = in ? g : G - 1;
+    const char* src = qbase + (gg * p.q.sh + tt * p.q.ss) * 2 + ll.hoff;
+    const uint32_t dst = lds0 + (i & 1) * C::QB + rw * BlockLayout<D>::BLOCK;
+#pragma unroll
+    for (int cp = 0; cp < C::PIECES / KW; ++cp) dma_global16(dst + (kw + KW * cp) * 1024, src + (kw + KW * cp) * 32);
+    if (C::PIECES < KW) {
+      if (kw < C::PIECES) dma_global16(dst + kw * 1024, src + kw * 32);
+    }
+    if (kw == 0 && hh == 0) {
+      mv = mbase[static_cast<int64_t>(gg) * p.T + tt];
+      pv = in && mv != -INFINITY ? first + tt : -1;
+    }
+    t += dt;
+    g += dg;
+    if (g >= G) {
+      g -= G;
+      ++t;
+    }
+  };
+  issue(0);
+
+  v8 kf[NK][ND16];
+#pragma unroll
+  for (int k = 0; k < NK; ++k) {
+    const int row = min(kbase + 32 * k + l32, L - 1);
+    const T* src = static_cast<const T*>(p.k.ptr) + b * p.k.sb + hk * p.k.sh + row * p.k.ss + 8 * hh;
+#pragma unroll
+    for (int ds = 0; ds < ND16; ++ds) kf[k][ds] = load16<v8>(src + ds * 16);
+  }
+  float sum[NK];
+#pragma unroll
+  for (int k = 0; k < NK; ++k) sum[k] = 0.f;
+  const RowBase<D> rb(l32, hh);
+
+  for (int i = 0; i < nst; ++i) {
+    if (kw == 0) {
+      if (hh == 0) {
+        ms[i & 1][32 * rw + ll.r] = mv;
+        ps[i & 1][32 * rw + ll.r] = pv;
+      }
+      const bool any = __any(hh == 0 && pv < 0);
+      if (lane == 0) odd[i & 1][rw] = any;
+    }
+    wait_vm<0>();     // this wave's share of the stage has landed
+    __syncthreads();  // and everyone's; everyone is done with the other buffers
+    if (i + 1 < nst) issue(i + 1);
+    const int row0 = rstart + i * C::ROWS + 32 * rw;
+    if (row0 >= R) continue;
+    const RowBase<D> qr = at_tile(rb, lds0 + (i & 1) * C::QB + rw * BlockLayout<D>::BLOCK);
+    f32x16 s[NK];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) s[k] = f32x16{};
+#pragma unroll
+    for (int ds = 0; ds < ND16; ++ds) {
+      const v8 qf = tile_read_row<D, v8>(qr, 0, ds);
+#pragma unroll
+      for (int k = 0; k < NK; ++k) s[k] = mfma32(qf, kf[k][ds], s[k]);
+    }
+    // every row of the block sees every key of the wave, but near the diagonal
+    const bool all = first + row0 / G >= kbase + 32 * NK - 1 && !odd[i & 1][rw];
+    if (all) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4_t m4 = *reinterpret_cast<const f32x4_t*>(&ms[i & 1][32 * rw + 8 * j + 4 * hh]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+          for (int k = 0; k < NK; ++k) {
+            const float x = s[k][4 * j + e];
+            sum[k] += fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -m4[e]));
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float m = ms[i & 1][32 * rw + 8 * j + 4 * hh + e];
+          const int pos = ps[i & 1][32 * rw + 8 * j + 4 * hh + e];
+#pragma unroll
+          for (int k = 0; k < NK; ++k) {
+            const float x = s[k][4 * j + e];
+            const float pr = fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -m));
+            sum[k] += pos >= kbase + 32 * k + l32 ? pr : 0.f;
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < NK; ++k) {
+    const float both = pair_sum(sum[k]);
+    if (hh == 0) part[wave][32 * k + l32] = both;
+  }
+  __syncthreads();
+  float* w = p.w + b * p.w_sb + hk * p.w_sh;
+  for (int e = tid; e < C::KEYS; e += C::NW * 64) {
+    const int key = key0 + e;
+    if (key >= L) break;
+    const int k_wave = e / (32 * NK), at = e - k_wave * 32 * NK;
+    float total = 0.f;
+#pragma unroll
+    for (int r = 0; r < RW; ++r) total += part[k_wave * RW + r][at];
+    w[key] += total;
+  }
+}
+
+namespace {
+
+template <typename T, int D, int KW, int RW, int NK>
+hipError_t launch_weights(const KeyWeightsParams& p, hipStream_t s) {
+  constexpr int KEYS = 32 * KW * NK;
+  const int ntiles = (p.cap + KEYS - 1) / KEYS;
+  const int blocks = p.B * p.Hkv * ntiles;
+  hipLaunchKernelGGL((key_weights_kernel<T, D, KW, RW, NK>), folded_grid(blocks, KW * RW * 64), dim3(KW * RW * 64), 0,
+                     s, p, ntiles, blocks);
+  return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_weights_t(const KeyWeightsParams& p, hipStream_t s) {
+  const int64_t rows = static_cast<int64_t>(p.Hq / p.Hkv) * p.T;
+  if (rows <= 32) return launch_weights<T, D, 4, 1, 1>(p, s);
+  return launch_weights<T, D, 2, 4, 1>(p, s);
+}
+
+template <typename T>
+hipError_t launch_weights_dt(const KeyWeightsParams& p, int D, hipStream_t s) {
+  switch (D) {
+    case 32: return launch_weights_t<T, 32>(p, s);
+    case 64: return launch_weights_t<T, 64>(p, s);
+    case 128: return launch_weights_t<T, 128>(p, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_key_weights(const KeyWeightsParams& p, int dtype, int D, hipStream_t stream) {
+  if (dtype == 0) return launch_weights_dt<__bf16>(p, D, stream);
+  return launch_weights_dt<_Float16>(p, D, stream);
+}
+
+}  // namespace ssa

@@ -27,6 +27,7 @@
 
 #include <cstring>
 
+#include "../../include/ssa_cache_ops.h"
 #include "../../include/ssa_mi355x.h"
 
 namespace {
@@ -43,6 +44,15 @@ struct Abi {
   decltype(&ssa_decode_workspace_bytes) decode_bytes;
 };
 Abi abi;
+
+struct CacheAbi {  // include/ssa_cache_ops.h
+  decltype(&ssa_tree_attention) tree;
+  decltype(&ssa_tree_workspace_bytes) tree_bytes;
+  decltype(&ssa_key_weights) key_weights;
+  decltype(&ssa_cache_evict) evict;
+  decltype(&ssa_cache_accept) accept;
+};
+CacheAbi cache_abi;
 
 constexpr int64_t kMaxRowStride = int64_t{1} << 24;
 
@@ -439,13 +449,205 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(address, ...): the C ABI entry points in the order of Abi
-PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != static_cast<Py_ssize_t>(sizeof(Abi) / sizeof(void*))) {
+// ------------------------------------------------------------ cache operators
+// A pair of caches, or one, and the lengths that go with it.
+struct Cache {
+  int64_t B, Hkv, cap, D;
+  int dtype;
+  bool ok(const at::Tensor& k, const at::Tensor& v, const at::Tensor& lens) {
+    if (k.dim() != 4 || k.sizes() != v.sizes() || k.numel() == 0 || k.scalar_type() != v.scalar_type()) return false;
+    B = k.size(0);
+    Hkv = k.size(1);
+    cap = k.size(2);
+    D = k.size(3);
+    dtype = dtype_code(k);
+    if ((dtype != SSA_DTYPE_BF16 && dtype != SSA_DTYPE_FP16) || (D != 32 && D != 64 && D != 128) ||
+        B > INT32_MAX || Hkv > INT32_MAX || cap > INT32_MAX)
+      return false;
+    return addressable(k, 2) && addressable(v, 2) && ints(lens, {B});
+  }
+  static bool ints(const at::Tensor& t, at::IntArrayRef size) {
+    return t.sizes() == size && t.scalar_type() == at::kInt && t.is_contiguous();
+  }
+  // q [B, Hq, T, D], or [B, Hq, D] for T = 1
+  bool queries(const at::Tensor& q, int64_t& Hq, int64_t& T, ssa_tensor4& view4) const {
+    const int64_t dim = q.dim();
+    if ((dim != 3 && dim != 4) || dtype_code(q) != dtype || q.numel() == 0 || q.size(0) != B || q.size(dim - 1) != D)
+      return false;
+    Hq = q.size(1);
+    T = dim == 4 ? q.size(2) : 1;
+    if (Hq % Hkv != 0 || Hq > INT32_MAX || T > INT32_MAX) return false;
+    if (q.stride(dim - 1) != 1 || (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) != 0) return false;
+    for (int64_t d = 0; d + 1 < dim; ++d)
+      if (q.size(d) > 1 && q.stride(d) % 8 != 0) return false;
+    if (dim == 4 && T > 1 && q.stride(2) >= kMaxRowStride) return false;
+    view4 = {q.data_ptr(), stride1(q, 0), stride1(q, 1), dim == 4 ? stride1(q, 2) : 0};
+    return true;
+  }
+  bool weights(const at::Tensor& w) const {
+    return w.dim() == 3 && w.size(0) == B && w.size(1) == Hkv && w.size(2) == cap && w.scalar_type() == at::kFloat &&
+           (cap == 1 || w.stride(2) == 1) && (B == 1 || w.stride(0) >= 0) && (Hkv == 1 || w.stride(1) >= 0);
+  }
+};
+
+int32_t i32(int64_t v) { return static_cast<int32_t>(v); }
+const int32_t* int_data(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
+at::Tensor int32s(at::IntArrayRef size, const at::Tensor& like) {
+  return at::empty(size, like.options().dtype(at::kInt));
+}
+bool cache_set() { return cache_abi.tree != nullptr; }
+
+// tree(q, k_cache, v_cache, lens, mask, scale, n, b, num_splits, return_m, dev, stream)
+//   -> (out, m) | (out,) | status | None
+PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12 || !cache_set()) return none();
+  Args in = args_of(a, n);
+  const at::Tensor *q = in.tensor(0), *k = in.tensor(1), *v = in.tensor(2), *lens = in.tensor(3), *mask = in.tensor(4);
+  const double scale = in.number(5);
+  const float *np = scalar(in.tensor(6)), *bp = scalar(in.tensor(7));
+  const int64_t splits = in.integer(8);
+  const bool with_m = a[9] == Py_True;
+  Cache c;
+  int64_t Hq, T;
+  ssa_tensor4 qv;
+  if (!in.good || np == nullptr || bp == nullptr || !c.ok(*k, *v, *lens) || !c.queries(*q, Hq, T, qv) || splits < 0 ||
+      splits > INT32_MAX || T > SSA_TREE_MAX_NODES)
+    return none();
+  if ((mask->scalar_type() != at::kBool && mask->scalar_type() != at::kByte) || !mask->is_contiguous()) return none();
+  const bool each = mask->dim() == 3;
+  if (each ? mask->sizes() != at::IntArrayRef({c.B, T, T}) : mask->sizes() != at::IntArrayRef({T, T})) return none();
+  at::Tensor out, m;
+  int32_t status;
+  {
+    pybind11::gil_scoped_release unlocked;
+    const bool rows = q->dim() == 4;
+    out = rows ? at::empty({c.B, Hq, T, c.D}, q->options()) : at::empty({c.B, Hq, c.D}, q->options());
+    if (with_m) m = rows ? floats({c.B, Hq, T}, *q) : floats({c.B, Hq}, *q);
+    const int64_t ws_bytes =
+        cache_abi.tree_bytes(i32(c.B), i32(Hq), i32(c.Hkv), i32(c.cap), i32(c.D), i32(T), i32(splits));
+    at::Tensor ws;
+    if (ws_bytes > 0) ws = bytes(ws_bytes, *q);
+    const ssa_tree_args f{qv, view(*k), view(*v),
+                          {out.data_ptr(), stride1(out, 0), stride1(out, 1), rows ? stride1(out, 2) : 0},
+                          with_m ? static_cast<float*>(m.data_ptr()) : nullptr, int_data(*lens),
+                          static_cast<const uint8_t*>(mask->data_ptr()), each ? T * T : 0, np, bp, i32(c.B), i32(Hq),
+                          i32(c.Hkv), i32(c.cap), i32(c.D), c.dtype, i32(T), i32(splits), static_cast<float>(scale),
+                          ws.defined() ? ws.data_ptr() : nullptr};
+    status = cache_abi.tree(&f, in.stream);
+  }
+  if (status != 0) return PyLong_FromLong(status);
+  return with_m ? pack({out, m}) : pack({out});
+  END_HANDLE_TH_ERRORS
+}
+
+// key_weights(q, k_cache, m, lens, weights, scale, n, b, dev, stream) -> () | status | None
+PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10 || !cache_set()) return none();
+  Args in = args_of(a, n);
+  const at::Tensor *q = in.tensor(0), *k = in.tensor(1), *m = in.tensor(2), *lens = in.tensor(3), *w = in.tensor(4);
+  const double scale = in.number(5);
+  const float *np = scalar(in.tensor(6)), *bp = scalar(in.tensor(7));
+  Cache c;
+  int64_t Hq, T;
+  ssa_tensor4 qv;
+  if (!in.good || np == nullptr || bp == nullptr || !c.ok(*k, *k, *lens) || !c.queries(*q, Hq, T, qv) || T > c.cap ||
+      !c.weights(*w))
+    return none();
+  if (m->scalar_type() != at::kFloat || !m->is_contiguous() ||
+      (m->sizes() != at::IntArrayRef({c.B, Hq, T}) && !(T == 1 && m->sizes() == at::IntArrayRef({c.B, Hq}))))
+    return none();
+  int32_t status;
+  {
+    pybind11::gil_scoped_release unlocked;
+    const ssa_key_weights_args f{qv, view(*k), static_cast<const float*>(m->data_ptr()),
+                                 static_cast<float*>(w->data_ptr()), w->stride(0), w->stride(1), int_data(*lens), np,
+                                 bp, i32(c.B), i32(Hq), i32(c.Hkv), i32(c.cap), i32(c.D), c.dtype, i32(T),
+                                 static_cast<float>(scale)};
+    status = cache_abi.key_weights(&f, in.stream);
+  }
+  if (status != 0) return PyLong_FromLong(status);
+  return pack({});
+  END_HANDLE_TH_ERRORS
+}
+
+// A cache that is written: no dimension of stride 0 (the library checks the rest).
+bool writable(const at::Tensor& t) {
+  for (int d = 0; d < 3; ++d)
+    if (t.size(d) > 1 && t.stride(d) <= 0) return false;
+  return true;
+}
+
+// evict(k_cache, v_cache, lens, weights, keep, sinks, recent, dev, stream)
+//   -> (lens, weights, kept) | status | None
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !cache_set()) return none();
+  Args in = args_of(a, n);
+  const at::Tensor *k = in.tensor(0), *v = in.tensor(1), *lens = in.tensor(2), *w = in.tensor(3);
+  const int64_t keep = in.integer(4), sinks = in.integer(5), recent = in.integer(6);
+  Cache c;
+  if (!in.good || !c.ok(*k, *v, *lens) || !c.weights(*w) || !writable(*k) || !writable(*v) ||
+      k->data_ptr() == v->data_ptr() || keep < 1 || keep > c.cap || sinks < 0 || recent < 0 || sinks > keep ||
+      recent > keep - sinks)
+    return none();
+  at::Tensor lens_out, w_out, kept;
+  int32_t status;
+  {
+    pybind11::gil_scoped_release unlocked;
+    lens_out = int32s({c.B}, *k);
+    w_out = floats({c.B, c.Hkv, c.cap}, *k);
+    kept = int32s({c.B, c.Hkv, keep}, *k);
+    const ssa_cache_evict_args f{view(*k), view(*v), static_cast<const float*>(w->data_ptr()), w->stride(0),
+                                 w->stride(1), int_data(*lens), static_cast<int32_t*>(lens_out.data_ptr()),
+                                 static_cast<float*>(w_out.data_ptr()), static_cast<int32_t*>(kept.data_ptr()),
+                                 i32(c.B), i32(c.Hkv), i32(c.cap), i32(c.D), c.dtype, i32(keep), i32(sinks),
+                                 i32(recent)};
+    status = cache_abi.evict(&f, in.stream);
+  }
+  if (status != 0) return PyLong_FromLong(status);
+  return pack({lens_out, w_out, kept});
+  END_HANDLE_TH_ERRORS
+}
+
+// accept(k_cache, v_cache, lens, path, accepted, nodes, dev, stream) -> (lens,) | status | None
+PyObject* accept(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || !cache_set()) return none();
+  Args in = args_of(a, n);
+  const at::Tensor *k = in.tensor(0), *v = in.tensor(1), *lens = in.tensor(2), *path = in.tensor(3),
+                   *accepted = in.tensor(4);
+  const int64_t nodes = in.integer(5);
+  Cache c;
+  if (!in.good || !c.ok(*k, *v, *lens) || !writable(*k) || !writable(*v) || k->data_ptr() == v->data_ptr() ||
+      path->dim() != 2 || nodes < 1 || nodes > SSA_TREE_MAX_NODES || path->size(1) < 1 || path->size(1) > nodes ||
+      !Cache::ints(*path, {c.B, path->size(1)}) || !Cache::ints(*accepted, {c.B}))
+    return none();
+  at::Tensor lens_out;
+  int32_t status;
+  {
+    pybind11::gil_scoped_release unlocked;
+    lens_out = int32s({c.B}, *k);
+    const ssa_cache_accept_args f{view(*k), view(*v), int_data(*lens), int_data(*path), int_data(*accepted),
+                                  static_cast<int32_t*>(lens_out.data_ptr()), i32(c.B), i32(c.Hkv), i32(c.cap),
+                                  i32(c.D), c.dtype, i32(nodes), i32(path->size(1))};
+    status = cache_abi.accept(&f, in.stream);
+  }
+  if (status != 0) return PyLong_FromLong(status);
+  return pack({lens_out});
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(address, ...): the C ABI entry points in the order of Abi;
+// bind_cache(address, ...): those of CacheAbi.
+template <typename Entries>
+PyObject* bind(Entries& to, PyObject* const* a, Py_ssize_t n) {
+  if (n != static_cast<Py_ssize_t>(sizeof(Entries) / sizeof(void*))) {
     PyErr_SetString(PyExc_TypeError, "bind: wrong number of entry points");
     return nullptr;
   }
-  void* p[sizeof(Abi) / sizeof(void*)];
+  void* p[sizeof(Entries) / sizeof(void*)];
   for (Py_ssize_t i = 0; i < n; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (p[i] == nullptr) {
@@ -453,12 +655,19 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return nullptr;
     }
   }
-  std::memcpy(&abi, p, sizeof(abi));
+  std::memcpy(&to, p, sizeof(to));
   Py_RETURN_NONE;
 }
+PyObject* bind_main(PyObject*, PyObject* const* a, Py_ssize_t n) { return bind(abi, a, n); }
+PyObject* bind_cache(PyObject*, PyObject* const* a, Py_ssize_t n) { return bind(cache_abi, a, n); }
 
 #define SSA_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr
-PyMethodDef methods[] = {{"bind", SSA_FAST(&bind)},
+PyMethodDef methods[] = {{"bind", SSA_FAST(&bind_main)},
+                         {"bind_cache", SSA_FAST(&bind_cache)},
+                         {"tree", SSA_FAST(&tree)},
+                         {"key_weights", SSA_FAST(&key_weights)},
+                         {"evict", SSA_FAST(&evict)},
+                         {"accept", SSA_FAST(&accept)},
                          {"fwd", SSA_FAST(&forward<false>)},
                          {"bwd", SSA_FAST(&backward<false>)},
                          {"varlen_fwd", SSA_FAST(&forward<true>)},
