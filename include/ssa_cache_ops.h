@@ -88,8 +88,15 @@ typedef struct ssa_key_weights_args {
   int32_t dtype;
   int32_t queries;      /* 1 .. capacity */
   float softmax_scale;
+  void* workspace;      /* ssa_key_weights_workspace_bytes() bytes, 16-byte aligned; may
+                           be NULL when that is 0 */
 } ssa_key_weights_args;
 
+/* Workspace bytes: a float per cached row and chunk of the queries where these
+   are split over workgroups (many queries of few heads), else 0; 0 on invalid
+   arguments. */
+int64_t ssa_key_weights_workspace_bytes(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t capacity,
+                                        int32_t queries);
 int32_t ssa_key_weights(const ssa_key_weights_args* args, void* stream);
 
 /*

@@ -57,6 +57,7 @@ EXPORTED_SYMBOLS = (
     "ssa_tree_num_splits",  # include/ssa_cache_ops.h
     "ssa_tree_workspace_bytes",
     "ssa_tree_attention",
+    "ssa_key_weights_workspace_bytes",
     "ssa_key_weights",
     "ssa_cache_evict",
     "ssa_cache_accept",
@@ -297,6 +298,7 @@ class KeyWeightsArgs(ctypes.Structure):
         ("dtype", ctypes.c_int32),
         ("queries", ctypes.c_int32),
         ("softmax_scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
     ]
 
 
@@ -385,6 +387,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ssa_tree_num_splits.argtypes = [i32] * 6
     lib.ssa_tree_workspace_bytes.restype = ctypes.c_int64
     lib.ssa_tree_workspace_bytes.argtypes = [i32] * 7
+    lib.ssa_key_weights_workspace_bytes.restype = ctypes.c_int64
+    lib.ssa_key_weights_workspace_bytes.argtypes = [i32] * 5
 
 
 def lib() -> ctypes.CDLL:
@@ -413,8 +417,8 @@ def lib() -> ctypes.CDLL:
 NATIVE_PATH = Path(__file__).resolve().parent / "_ssa_native.so"
 _NATIVE_ENTRIES = ("ssa_fwd", "ssa_bwd", "ssa_varlen_fwd", "ssa_varlen_bwd", "ssa_decode", "ssa_bwd_partials_count",
                    "ssa_bwd_ds_workspace_bytes", "ssa_varlen_bwd_ds_workspace_bytes", "ssa_decode_workspace_bytes")
-_NATIVE_CACHE_ENTRIES = ("ssa_tree_attention", "ssa_tree_workspace_bytes", "ssa_key_weights", "ssa_cache_evict",
-                         "ssa_cache_accept")
+_NATIVE_CACHE_ENTRIES = ("ssa_tree_attention", "ssa_tree_workspace_bytes", "ssa_key_weights",
+                         "ssa_key_weights_workspace_bytes", "ssa_cache_evict", "ssa_cache_accept")
 _native = None
 
 

@@ -213,10 +213,12 @@ def ssa_key_weights(q, k_cache, m, cache_seqlens, weights, softmax_scale, ssa_n,
     _check_weights(weights, B, Hkv, cap, q.device)
     lens = _lens(cache_seqlens, B, q.device)
     n32, b32 = _scalar(ssa_n, q.device), _scalar(ssa_b, q.device)
+    ws_bytes = int(_lib.lib().ssa_key_weights_workspace_bytes(B, Hq, Hkv, cap, T))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes > 0 else None
     args = _lib.KeyWeightsArgs(
         _t4(q4), _t4(k_cache), m32.data_ptr(), weights.data_ptr(), weights.stride(0), weights.stride(1),
         lens.data_ptr(), n32.data_ptr(), b32.data_ptr(), B, Hq, Hkv, cap, D, _DTYPES[q.dtype], T,
-        float(softmax_scale),
+        float(softmax_scale), ws.data_ptr() if ws is not None else None,
     )
     _launch("ssa_key_weights", args, q.device)
     return weights

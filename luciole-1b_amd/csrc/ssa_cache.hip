@@ -3,7 +3,7 @@
 //
 // Eviction keeps `keep` rows of each (sequence, kv-head).  evict_select_kernel
 // finds the weight of the last row that stays by a radix selection over the
-// weights' bits in an order-preserving form (three histograms of 11, 11 and 10
+// weights' bits in an order-preserving form (three histograms of 12, 10 and 10
 // bits), then writes the kept rows' indices and weights in ascending order: a
 // row's place is the number of rows before it that stay, that is of rows above
 // the threshold plus the smaller of the rows at it and the number of those that
@@ -20,7 +20,9 @@ namespace ssa {
 namespace {
 
 constexpr int kSelect = 1024;  // threads of a selection
-constexpr int kBins = 2048;
+constexpr int kBins = 4096;
+
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 
 // Unsigned order of weights: NaN below everything, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_bits(float w) {
@@ -59,6 +61,10 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* waves, int 
 
 }  // namespace
 
+// E rows a thread at a time, four consecutive ones per 4096: a cache of up to
+// 1024 E rows is read once and stays in registers for every pass, a longer one
+// is read in such stretches by each of the four.
+template <int E>
 __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams p, int nblocks) {
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t waves[kSelect / 64];
@@ -77,81 +83,112 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams p, in
     for (int i = tid; i < p.keep; i += kSelect) kept[i] = i < L ? i : -1;
     return;
   }
+  for (int i = p.keep + tid; i < p.cap; i += kSelect) w_out[i] = 0.f;
+  constexpr int STRETCH = kSelect * E;
+  float v[E];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int j = 0; j < E / 4; ++j) {
+      const int i = r0 + 4 * kSelect * j + 4 * tid;
+      if (i + 3 < L) {
+        const f32x4_u x = *reinterpret_cast<const f32x4_u*>(w + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * j + e] = x[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * j + e] = i + e < L ? w[i + e] : 0.f;
+      }
+    }
+  };
+  const bool once = L <= STRETCH;
+  if (once) load(0);
   // rows [lo, hi) are chosen from; sinks + recent <= keep < L, so lo < hi
   const int lo = p.sinks, hi = L - p.recent;
   uint32_t need = p.keep - p.sinks - p.recent;  // of them stay, fewer than there are
-  uint32_t prefix = 0, ties = 0;
+  uint32_t prefix = 0;
   const bool choose = need > 0;
   if (choose) {
-    constexpr int kShift[3] = {21, 10, 0}, kWidth[3] = {11, 11, 10};
+    constexpr int kShift[3] = {20, 10, 0}, kWidth[3] = {12, 10, 10};
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
-      for (int i = tid; i < kBins; i += kSelect) hist[i] = 0;
+      const int bins = 1 << kWidth[pass];
+      for (int i = tid; i < bins; i += kSelect) hist[i] = 0;
       __syncthreads();
-      const int shift = kShift[pass];
-      const uint32_t mask = (1u << kWidth[pass]) - 1u;
-      for (int i = lo + tid; i < hi; i += kSelect) {
-        const uint32_t key = order_bits(w[i]);
-        if (pass == 0 || (key >> (shift + kWidth[pass])) == prefix) atomicAdd(&hist[(key >> shift) & mask], 1u);
+      for (int r0 = 0; r0 < L; r0 += STRETCH) {
+        if (!once) load(r0);
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const int i = r0 + 4 * kSelect * (j / 4) + 4 * tid + j % 4;
+          const uint32_t key = order_bits(v[j]);
+          if (i >= lo && i < hi && (pass == 0 || (key >> (kShift[pass] + kWidth[pass])) == prefix))
+            atomicAdd(&hist[(key >> kShift[pass]) & (bins - 1)], 1u);
+        }
       }
       __syncthreads();
-      // bins from the top: thread i takes bins 2047 - 2 i and the one below
-      const uint32_t h0 = hist[kBins - 1 - 2 * tid], h1 = hist[kBins - 2 - 2 * tid];
+      // bins from the top: thread i takes `per` bins downwards from the i-th group
+      const int per = bins / kSelect;
+      uint32_t mine = 0;
+      for (int x = 0; x < per; ++x) mine += hist[bins - 1 - per * tid - x];
       uint32_t total;
-      const uint32_t upto = block_scan(h0 + h1, waves, tid, total);
-      const uint32_t above = upto - h0 - h1;
+      const uint32_t upto = block_scan(mine, waves, tid, total);
+      uint32_t above = upto - mine;
       if (above < need && upto >= need) {
-        const bool second = above + h0 < need;
-        found[0] = kBins - 1 - 2 * tid - (second ? 1 : 0);
-        found[1] = second ? above + h0 : above;
+        int bin = bins - 1 - per * tid;
+        while (above + hist[bin] < need) above += hist[bin--];
+        found[0] = bin;
+        found[1] = above;
       }
       __syncthreads();
       prefix = (prefix << kWidth[pass]) | found[0];
       need -= found[1];
     }
-    ties = need;  // rows at the threshold that stay, the lowest first
   }
-  // places: 4 consecutive rows a thread
+  const uint32_t ties = need;  // rows at the threshold that stay, the lowest first
   uint32_t above0 = 0, at0 = 0;  // rows before this stretch that surely stay; at the threshold
-  for (int r0 = 0; r0 < L; r0 += 4 * kSelect) {
-    float v[4];
-    uint32_t up[4], eq[4], count = 0;
+  for (int r0 = 0; r0 < L; r0 += STRETCH) {
+    if (!once) load(r0);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = r0 + 4 * tid + e;
-      v[e] = i < L ? w[i] : 0.f;
-      const uint32_t key = order_bits(v[e]);
-      const bool inside = i >= lo && i < hi;
-      up[e] = i < L && (!inside || (choose && key > prefix));
-      eq[e] = inside && choose && key == prefix;
-      count += up[e] + (eq[e] << 16);
-    }
-    uint32_t total;
-    uint32_t before = block_scan(count, waves, tid, total) - count;  // both below 2^13: no carry
+    for (int j = 0; j < E / 4; ++j) {
+      const int first = r0 + 4 * kSelect * j;
+      if (first >= L) break;
+      uint32_t up[4], eq[4], count = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t at = at0 + (before >> 16), place = above0 + (before & 0xffffu) + (at < ties ? at : ties);
-      if (up[e] || (eq[e] && at < ties)) {
-        kept[place] = r0 + 4 * tid + e;
-        w_out[place] = v[e];
+      for (int e = 0; e < 4; ++e) {
+        const int i = first + 4 * tid + e;
+        const uint32_t key = order_bits(v[4 * j + e]);
+        const bool inside = i >= lo && i < hi;
+        up[e] = i < L && (!inside || (choose && key > prefix));
+        eq[e] = inside && choose && key == prefix;
+        count += up[e] + (eq[e] << 16);
       }
-      before += up[e] + (eq[e] << 16);
+      uint32_t total;
+      uint32_t before = block_scan(count, waves, tid, total) - count;  // both at most 2^12: no carry
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t at = at0 + (before >> 16), place = above0 + (before & 0xffffu) + (at < ties ? at : ties);
+        if (up[e] || (eq[e] && at < ties)) {
+          kept[place] = first + 4 * tid + e;
+          w_out[place] = v[4 * j + e];
+        }
+        before += up[e] + (eq[e] << 16);
+      }
+      above0 += total & 0xffffu;
+      at0 += total >> 16;
     }
-    above0 += total & 0xffffu;
-    at0 += total >> 16;
   }
-  for (int i = p.keep + tid; i < p.cap; i += kSelect) w_out[i] = 0.f;
 }
 
-// One workgroup per (tensor, sequence, kv-head, slice of SP 16-byte pieces of a row).
+// One workgroup per (tensor, sequence, kv-head, slice of SP 16-byte pieces of a
+// row), the slices of a head on one XCD.  The next chunk's rows are on their way
+// while this one's are written.
 template <int SP>
 __global__ __launch_bounds__(1024) void evict_move_kernel(EvictParams p, int slices, int nblocks) {
   constexpr int U = 4, ROWS = 1024 / SP;  // rows of one step, U steps a chunk
   const int block = folded_block();
   if (block >= nblocks) return;
-  int u = block;
-  const int slice = u % slices;
-  u /= slices;
+  const int units = nblocks / slices;
+  const int slice = block / units;
+  int u = block - slice * units;
   const Tensor4& t = (u & 1) ? p.v : p.k;
   u >>= 1;
   const int h = u % p.Hkv, b = u / p.Hkv;
@@ -160,22 +197,37 @@ __global__ __launch_bounds__(1024) void evict_move_kernel(EvictParams p, int sli
   const int* kept = p.kept + static_cast<int64_t>(u) * p.keep;
   const int tid = threadIdx.x, piece = slice * SP + tid % SP, row = tid / SP;
   char* base = static_cast<char*>(const_cast<void*>(t.ptr)) + (b * t.sb + h * t.sh) * 2 + piece * 16;
+  const int64_t step = t.ss * 2;
+  u32x4 v[U], next[U];
+  int src[U];
+  auto index = [&](int r0) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int r = r0 + j * ROWS + row;
+      src[j] = r < p.keep ? kept[r] : r;
+    }
+  };
+  auto fetch = [&](u32x4 (&to)[U], int r0) {
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (src[j] != r0 + j * ROWS + row) to[j] = *reinterpret_cast<const u32x4*>(base + src[j] * step);
+  };
+  index(0);
+  fetch(v, 0);
   for (int r0 = 0; r0 < p.keep; r0 += U * ROWS) {
-    u32x4 v[U];
     bool moves[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int r = r0 + j * ROWS + row;
-      const int src = r < p.keep ? kept[r] : r;
-      moves[j] = src != r;
-      if (moves[j]) v[j] = *reinterpret_cast<const u32x4*>(base + static_cast<int64_t>(src) * t.ss * 2);
-    }
+    for (int j = 0; j < U; ++j) moves[j] = src[j] != r0 + j * ROWS + row;
+    const bool more = r0 + U * ROWS < p.keep;
+    if (more) index(r0 + U * ROWS);
     __builtin_amdgcn_s_waitcnt(0);  // the chunk's rows are in registers ...
     __syncthreads();                // ... everywhere
+    if (more) fetch(next, r0 + U * ROWS);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int r = r0 + j * ROWS + row;
-      if (moves[j]) *reinterpret_cast<u32x4*>(base + static_cast<int64_t>(r) * t.ss * 2) = v[j];
+      if (moves[j]) *reinterpret_cast<u32x4*>(base + r * step) = v[j];
+      v[j] = next[j];
     }
   }
 }
@@ -225,7 +277,13 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptParams p, int sp, int
 
 hipError_t launch_evict(const EvictParams& p, hipStream_t s) {
   const int heads = p.B * p.Hkv;
-  hipLaunchKernelGGL(evict_select_kernel, folded_grid(heads, kSelect), dim3(kSelect), 0, s, p, heads);
+  const dim3 grid = folded_grid(heads, kSelect);
+  if (p.cap <= 4 * kSelect)
+    hipLaunchKernelGGL(evict_select_kernel<4>, grid, dim3(kSelect), 0, s, p, heads);
+  else if (p.cap <= 16 * kSelect)
+    hipLaunchKernelGGL(evict_select_kernel<16>, grid, dim3(kSelect), 0, s, p, heads);
+  else
+    hipLaunchKernelGGL(evict_select_kernel<32>, grid, dim3(kSelect), 0, s, p, heads);
   const int slices = p.D / 8 / 4;  // 64-byte slices
   const int blocks = heads * 2 * slices;
   hipLaunchKernelGGL((evict_move_kernel<4>), folded_grid(blocks, 1024), dim3(1024), 0, s, p, slices, blocks);

@@ -75,6 +75,11 @@ bool tree_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t cap, int32_t T, int32_t
   return ssa::tree_units(B, Hq, Hkv, T) * splits < (1ll << 30);
 }
 
+bool weights_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t cap, int32_t T) {
+  // at most 2^28 * 4 workgroups
+  return cache_ok(B, Hkv, cap) && rows_ok(B, Hq, Hkv, T) && T <= cap;
+}
+
 int64_t tree_ml_floats(int64_t recs) { return (2 * recs + 3) & ~static_cast<int64_t>(3); }
 
 Tensor4 to_t4(const ssa_tensor4& t) { return Tensor4{t.ptr, t.stride_b, t.stride_h, t.stride_s}; }
@@ -114,6 +119,7 @@ int32_t ssa_tree_attention(const ssa_tree_args* a, void* stream) {
   if (a->mask_stride_b < 0) return SSA_ERR_ALIGNMENT;
   ssa::TreeParams p{};
   p.splits = ssa::tree_splits(a->batch, a->heads_q, a->heads_kv, a->capacity, a->nodes, a->num_splits);
+  p.split_keys = ssa::tree_split_keys(a->batch, a->heads_q, a->heads_kv, a->capacity, a->nodes, a->num_splits);
   if (p.splits > 1) {
     if (a->workspace == nullptr) return SSA_ERR_NULL_POINTER;
     if (!aligned16(a->workspace)) return SSA_ERR_ALIGNMENT;
@@ -140,11 +146,16 @@ int32_t ssa_tree_attention(const ssa_tree_args* a, void* stream) {
   return launch_status(ssa::launch_tree(p, a->dtype, a->head_dim, static_cast<hipStream_t>(stream)));
 }
 
+int64_t ssa_key_weights_workspace_bytes(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t capacity,
+                                        int32_t queries) {
+  if (!weights_ok(batch, heads_q, heads_kv, capacity, queries)) return 0;
+  const int64_t chunks = ssa::weights_chunks(batch, heads_q, heads_kv, capacity, queries);
+  return chunks > 1 ? chunks * batch * heads_kv * capacity * 4 : 0;
+}
+
 int32_t ssa_key_weights(const ssa_key_weights_args* a, void* stream) {
   if (a == nullptr) return SSA_ERR_NULL_POINTER;
-  if (!cache_ok(a->batch, a->heads_kv, a->capacity) || !rows_ok(a->batch, a->heads_q, a->heads_kv, a->queries) ||
-      a->queries > a->capacity)
-    return SSA_ERR_SHAPE;
+  if (!weights_ok(a->batch, a->heads_q, a->heads_kv, a->capacity, a->queries)) return SSA_ERR_SHAPE;
   SSA_TRY(check_types(a->head_dim, a->dtype));
   SSA_TRY(check_tensor(a->q));
   SSA_TRY(check_tensor(a->k_cache));
@@ -156,6 +167,13 @@ int32_t ssa_key_weights(const ssa_key_weights_args* a, void* stream) {
   if (!disjoint({nullptr, a->weights_stride_b, a->weights_stride_h, 0}, a->batch, a->heads_kv, 1, a->capacity))
     return SSA_ERR_ALIGNMENT;
   ssa::KeyWeightsParams p{};
+  p.chunks = ssa::weights_chunks(a->batch, a->heads_q, a->heads_kv, a->capacity, a->queries);
+  p.chunk_rows = ssa::weights_chunk_rows(static_cast<int64_t>(a->heads_q / a->heads_kv) * a->queries, p.chunks);
+  if (p.chunks > 1) {
+    if (a->workspace == nullptr) return SSA_ERR_NULL_POINTER;
+    if (!aligned16(a->workspace)) return SSA_ERR_ALIGNMENT;
+    p.ws = static_cast<float*>(a->workspace);
+  }
   p.q = to_t4(a->q);
   p.k = to_t4(a->k_cache);
   p.m = a->m;

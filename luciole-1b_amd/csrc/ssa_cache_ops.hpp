@@ -19,7 +19,8 @@ struct TreeParams {
   const float* b_ptr;
   float* ws_ml;   // [B * Hq * T * splits][2]
   float* ws_acc;  // [B * Hq * T * splits][D]
-  int B, Hq, Hkv, cap, T, splits;
+  int B, Hq, Hkv, cap, T;
+  int splits, split_keys;  // split s: keys s * split_keys ..
   float scale;
 };
 
@@ -31,7 +32,9 @@ struct KeyWeightsParams {
   const int* seqlens;
   const float* n_ptr;
   const float* b_ptr;
+  float* ws;  // chunks > 1: [chunks][B * Hkv][cap]
   int B, Hq, Hkv, cap, T;
+  int chunks, chunk_rows;  // the rows (queries of all heads of a group) of one chunk
   float scale;
 };
 
@@ -65,17 +68,39 @@ inline int64_t tree_units(int B, int Hq, int Hkv, int T) {
   return static_cast<int64_t>(B) * Hkv * ((rows + per - 1) / per);
 }
 
-inline int tree_splits(int B, int Hq, int Hkv, int cap, int T, int requested) {
-  const int64_t most = (cap + 127ll) / 128;
+// Keys of a split (a multiple of 256, the steps of every kernel) for a wanted
+// number of splits, and the splits of that length.
+constexpr int kTreeStep = 256;
+inline int tree_split_keys(int B, int Hq, int Hkv, int cap, int T, int requested) {
   int64_t want = requested;
   if (want <= 0) {
     const int64_t units = tree_units(B, Hq, Hkv, T);
     want = (256 + units - 1) / units;
-    const int64_t longest = (cap + 255ll) / 256;
-    if (want > longest) want = longest;
   }
-  if (want > most) want = most;
-  return static_cast<int>(want < 1 ? 1 : want);
+  const int64_t keys = (cap + want - 1) / want;
+  return static_cast<int>((keys + kTreeStep - 1) / kTreeStep * kTreeStep);
+}
+inline int tree_splits(int B, int Hq, int Hkv, int cap, int T, int requested) {
+  const int keys = tree_split_keys(B, Hq, Hkv, cap, T, requested);
+  return static_cast<int>((static_cast<int64_t>(cap) + keys - 1) / keys);
+}
+
+// Key weights of more than 32 rows: rows of a stage and keys of a workgroup.
+constexpr int kWeightsStage = 128;
+constexpr int kWeightsKeys = 64;
+// Chunks of the rows: about 2048 workgroups in all, so that those of many rows
+// and of few even out, of 1024 rows at least.
+inline int weights_chunks(int B, int Hq, int Hkv, int cap, int T) {
+  const int64_t rows = static_cast<int64_t>(Hq / Hkv) * T;
+  if (rows <= 32) return 1;
+  const int64_t blocks = static_cast<int64_t>(B) * Hkv * ((cap + kWeightsKeys - 1) / kWeightsKeys);
+  const int64_t want = 2048 / blocks, most = rows / 1024;
+  const int64_t n = want < most ? want : most;
+  return static_cast<int>(n < 1 ? 1 : n);
+}
+inline int weights_chunk_rows(int64_t rows, int chunks) {
+  const int64_t per = (rows + chunks - 1) / chunks;
+  return static_cast<int>((per + kWeightsStage - 1) / kWeightsStage * kWeightsStage);
 }
 
 hipError_t launch_tree(const TreeParams& p, int dtype, int D, hipStream_t stream);

@@ -11,7 +11,9 @@
 // The G heads of a group and their T queries are rows r = t * G + head, so the
 // causal mask only bounds the first row of a workgroup's keys and the rows
 // near it.  A workgroup is KW key waves of 32 NK keys by RW row waves of 32
-// rows; Q rows pass through LDS in stages of 32 RW rows, two in flight.
+// rows; Q rows pass through LDS in stages of 32 RW rows, two in flight.  Many
+// rows are split over workgroups in chunks, whose sums a second kernel adds up
+// in their order.
 #include "ssa_cache_ops.hpp"
 #include "ssa_common.hpp"
 #include "ssa_launch.hpp"
@@ -29,6 +31,13 @@ struct WeightsCfg {
   static constexpr int QB = ROWS * D * 2;           // bytes of its Q rows
   static constexpr int PIECES = BlockLayout<D>::IPB;  // 1 KB pieces of a 32-row block
 };
+
+__device__ __forceinline__ int clamped_length(const KeyWeightsParams& p, int b) {
+  const int L = load_table_entry(p.seqlens, b);
+  return L < 0 ? 0 : (L > p.cap ? p.cap : L);
+}
+// The first row whose query stands at `key` or behind it.
+__device__ __forceinline__ int first_row(int key, int first, int G) { return key > first ? (key - first) * G : 0; }
 
 }  // namespace
 
@@ -48,25 +57,30 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
   if (block >= nblocks) return;
   // all (sequence, head) pairs of a key tile together: the tiles of most rows come first
   const int nbh = p.B * p.Hkv;
-  const int tile = block / nbh, bh = block - tile * nbh;
+  const int chunk = block / (nbh * ntiles);
+  const int tile = (block - chunk * nbh * ntiles) / nbh, bh = block % nbh;
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
-  int L = load_table_entry(p.seqlens, b);
-  L = L < 0 ? 0 : (L > p.cap ? p.cap : L);
+  const int L = clamped_length(p, b);
   const int key0 = tile * C::KEYS;
   if (key0 >= L) return;
+  const int G = p.Hq / p.Hkv, first = L - p.T;  // first: position of query 0
+  // rows from the stage of the first query that sees key0 on; those of the chunk
+  const int64_t chunk0 = static_cast<int64_t>(chunk) * p.chunk_rows;
+  const int R = static_cast<int>(min(static_cast<int64_t>(G) * p.T, chunk0 + p.chunk_rows));
+  const int sees = first_row(key0, first, G) / C::ROWS * C::ROWS;
+  const int rstart = max(sees, static_cast<int>(chunk0));
+  if (rstart >= R) return;  // of the key's other chunks
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kw = wave / RW, rw = wave - kw * RW;
   const int l32 = lane & 31, hh = lane >> 5;
-  const int G = p.Hq / p.Hkv, R = G * p.T, first = L - p.T;  // first: position of query 0
   const float n = *p.n_ptr, c = p.scale * *p.b_ptr;
   const int kbase = key0 + 32 * NK * kw;  // this wave's keys
 
-  // rows from the first query that sees key0 on
-  const int tstart = key0 > first ? key0 - first : 0;
-  const int rstart = tstart * G;  // < R: key0 < L
   const int nst = (R - rstart + C::ROWS - 1) / C::ROWS;
+  // rows of whole blocks that see every key of the wave
+  const int rall = first_row(kbase + 32 * NK - 1, first, G);
 
   // the row of its block that this lane's loads fetch, as (query, head), moved
   // on by one stage at a time
@@ -95,6 +109,7 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
     }
     if (kw == 0 && hh == 0) {
       mv = mbase[static_cast<int64_t>(gg) * p.T + tt];
+      // chunks end with a stage, so a row past R is past the last query
       pv = in && mv != -INFINITY ? first + tt : -1;
     }
     t += dt;
@@ -144,7 +159,7 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
       for (int k = 0; k < NK; ++k) s[k] = mfma32(qf, kf[k][ds], s[k]);
     }
     // every row of the block sees every key of the wave, but near the diagonal
-    const bool all = first + row0 / G >= kbase + 32 * NK - 1 && !odd[i & 1][rw];
+    const bool all = row0 >= rall && !odd[i & 1][rw];
     if (all) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -181,7 +196,8 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
     if (hh == 0) part[wave][32 * k + l32] = both;
   }
   __syncthreads();
-  float* w = p.w + b * p.w_sb + hk * p.w_sh;
+  float* w = p.chunks == 1 ? p.w + b * p.w_sb + hk * p.w_sh
+                           : p.ws + (static_cast<int64_t>(chunk) * nbh + bh) * p.cap;
   for (int e = tid; e < C::KEYS; e += C::NW * 64) {
     const int key = key0 + e;
     if (key >= L) break;
@@ -189,19 +205,41 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
     float total = 0.f;
 #pragma unroll
     for (int r = 0; r < RW; ++r) total += part[k_wave * RW + r][at];
-    w[key] += total;
+    w[key] = p.chunks == 1 ? w[key] + total : total;
   }
+}
+
+// The chunks' sums of each key, in order.  KEYS, ROWS: those of the kernel that made them.
+template <int KEYS, int ROWS>
+__global__ __launch_bounds__(256) void key_weights_join_kernel(KeyWeightsParams p, int blocks_per_head, int nblocks) {
+  const int block = folded_block();
+  if (block >= nblocks) return;
+  const int bh = block / blocks_per_head, key = (block - bh * blocks_per_head) * 256 + threadIdx.x;
+  const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const int L = clamped_length(p, b);
+  if (key >= L) return;
+  const int sees = first_row(key / KEYS * KEYS, L - p.T, p.Hq / p.Hkv) / ROWS * ROWS;
+  const int64_t nbh = static_cast<int64_t>(p.B) * p.Hkv;
+  float total = 0.f;
+  for (int c = sees / p.chunk_rows; c < p.chunks; ++c) total += p.ws[(c * nbh + bh) * p.cap + key];
+  p.w[b * p.w_sb + hk * p.w_sh + key] += total;
 }
 
 namespace {
 
 template <typename T, int D, int KW, int RW, int NK>
 hipError_t launch_weights(const KeyWeightsParams& p, hipStream_t s) {
-  constexpr int KEYS = 32 * KW * NK;
-  const int ntiles = (p.cap + KEYS - 1) / KEYS;
-  const int blocks = p.B * p.Hkv * ntiles;
-  hipLaunchKernelGGL((key_weights_kernel<T, D, KW, RW, NK>), folded_grid(blocks, KW * RW * 64), dim3(KW * RW * 64), 0,
-                     s, p, ntiles, blocks);
+  using C = WeightsCfg<D, KW, RW, NK>;
+  const int ntiles = (p.cap + C::KEYS - 1) / C::KEYS;
+  const int heads = p.B * p.Hkv;
+  const int blocks = heads * ntiles * p.chunks;
+  hipLaunchKernelGGL((key_weights_kernel<T, D, KW, RW, NK>), folded_grid(blocks, C::NW * 64), dim3(C::NW * 64), 0, s,
+                     p, ntiles, blocks);
+  if (p.chunks > 1) {
+    const int per = (p.cap + 255) / 256;
+    hipLaunchKernelGGL((key_weights_join_kernel<C::KEYS, C::ROWS>), folded_grid(heads * per, 256), dim3(256), 0, s, p,
+                       per, heads * per);
+  }
   return hipGetLastError();
 }
 
@@ -209,7 +247,7 @@ template <typename T, int D>
 hipError_t launch_weights_t(const KeyWeightsParams& p, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(p.Hq / p.Hkv) * p.T;
   if (rows <= 32) return launch_weights<T, D, 4, 1, 1>(p, s);
-  return launch_weights<T, D, 2, 4, 1>(p, s);
+  return launch_weights<T, D, 2, kWeightsStage / 32, kWeightsKeys / 64>(p, s);
 }
 
 template <typename T>

@@ -18,9 +18,16 @@
 //     wave streams its own tiles of 32 keys through a private LDS ring, for one
 //     or two groups of 32 rows at once, and the waves merge at the end;
 //   * more (tree_wide_kernel): the transform (one log2 and one exp2 a pair) is
-//     the bound; 4 or 8 waves of 32 rows share each stage of 64 keys.
-// The keys are split over workgroups by the sequence's own length; partials
-// (m, l, acc) meet in split order in tree_merge_kernel.
+//     the bound; QW groups of 32 rows by KW key waves share each stage of keys,
+//     and the key waves merge at the end.
+// The keys are split over workgroups in ranges of one length for all sequences
+// (a ragged batch is then a number of equal pieces of work, and a sequence's
+// result does not depend on the others); partials (m, l, acc) meet in split
+// order in tree_merge_kernel.
+//
+// The running maximum is moved only when a lane's sum of a tile passes a bound
+// with the old one (kTreeSum): the rescaling of acc and the tile's maximum are
+// then rare, a quarter of the vector work.
 //
 // The mask is packed to one bit per node when a workgroup's keys reach the
 // tree's rows; tiles before them do no mask work.
@@ -36,6 +43,14 @@ namespace {
 
 constexpr int kMaxNodes = 1024;
 constexpr int kMaskWords = kMaxNodes / 32 + 1;  // words of a packed mask row, one of padding
+// A lane's sum of 16 p with the old maximum: below it no p overflows fp16, and
+// sums of 2^30 keys stay far from fp32's range.
+constexpr float kTreeSum = 16384.f;
+
+__device__ __forceinline__ int clamped_length(const TreeParams& p, int b) {
+  const int L = load_table_entry(p.seqlens, b);
+  return L < 0 ? 0 : (L > p.cap ? p.cap : L);
+}
 
 // What a workgroup works on.
 struct TreeUnit {
@@ -43,26 +58,25 @@ struct TreeUnit {
   int G, base, kbeg, kend, ntile;
   const char* kg;
   const char* vg;
-  __device__ __forceinline__ TreeUnit(const TreeParams& p, int block, int per, int nqb, int step) {
+  __device__ __forceinline__ TreeUnit(const TreeParams& p, int block, int per, int nqb) {
     int u = block;
-    split = u % p.splits;
-    u /= p.splits;
-    const int qb = u % nqb;
-    u /= nqb;
-    hk = u % p.Hkv;
+    // the splits' first ranges of all sequences, then the second ones ...: the
+    // short last ranges come late
+    const int nbh = p.B * p.Hkv, whole = nbh * nqb;
+    split = u / whole;
+    u -= split * whole;
+    const int qb = u / nbh;
+    u -= qb * nbh;
     b = u / p.Hkv;
+    hk = u - b * p.Hkv;
     G = p.Hq / p.Hkv;
     row0 = qb * per;
     nrows = min(per, G * p.T - row0);
-    int L = load_table_entry(p.seqlens, b);
-    L = L < 0 ? 0 : (L > p.cap ? p.cap : L);
+    const int L = clamped_length(p, b);
     base = L - p.T;
-    // the sequence's own keys over the splits, in whole steps
-    const int64_t per_split = (static_cast<int64_t>(L) + p.splits - 1) / p.splits;
-    const int64_t keys = (per_split + step - 1) / step * step;
-    const int64_t beg = split * keys;
+    const int64_t beg = static_cast<int64_t>(split) * p.split_keys;
     kbeg = beg < L ? static_cast<int>(beg) : L;
-    kend = beg + keys < L ? static_cast<int>(beg + keys) : L;
+    kend = beg + p.split_keys < L ? static_cast<int>(beg + p.split_keys) : L;
     ntile = (kend - kbeg + 31) / 32;
     kg = static_cast<const char*>(p.k.ptr) + (b * p.k.sb + hk * p.k.sh) * 2;
     vg = static_cast<const char*>(p.v.ptr) + (b * p.v.sb + hk * p.v.sh) * 2;
@@ -193,6 +207,21 @@ __device__ __forceinline__ void tree_tile(const RowBase<D>& kr, const TrBase<D>&
   v8 pb[NQ][2];
 #pragma unroll
   for (int g = 0; g < NQ; ++g) {
+    if constexpr (!MASKED) {
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = s[g][r];
+        const float pv = fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -st[g].m));
+        sum += pv;
+        pb[g][r >> 3][r & 7] = static_cast<T>(pv);
+      }
+      // m = -inf (nothing seen yet) gives an infinite or NaN sum
+      if (__builtin_expect(__all(sum <= kTreeSum), 1)) {
+        st[g].l += sum;
+        continue;
+      }
+    }
     float z = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -294,15 +323,15 @@ __device__ __forceinline__ void tree_stream_body(const TreeParams& p, char* smem
     block_load_wave<D>(u.kg, p.k.ss, row0, u.kend, dst, lk0, lk1);
     block_load_wave<D>(u.vg, p.v.ss, row0, u.kend, dst + C::BLOCK, lv0, lv1);
   };
+  if (ntw > 0) {
+#pragma unroll
+    for (int i = 0; i < NB - 1; ++i) issue(i);
+  }
   RowGroup<T, D> st[NQ];
 #pragma unroll
   for (int g = 0; g < NQ; ++g) st[g].init(p, u, 32 * g + l32, hh);
   const bool reaches = u.kend > u.kbeg && u.kend > u.base;
   if (reaches) pack_mask(p, u, words, tid, NW * 64);
-  if (ntw > 0) {
-#pragma unroll
-    for (int i = 0; i < NB - 1; ++i) issue(i);
-  }
   __syncthreads();
   if (ntw > 0) {
     const int W = mask_stride(p.T), n0 = u.row0 / u.G;
@@ -380,65 +409,109 @@ __device__ __forceinline__ void tree_stream_body(const TreeParams& p, char* smem
 }
 
 // ------------------------------------------------------------ more than 64 rows
-// 64 keys a stage, K block pairs then V block pairs, two stages.
-template <int D, int QW>
+// Two stages of 32 KW U keys, a K tile and a V tile each; wave (qw, kw) takes
+// the stage's key tiles kw, kw + KW, ...
+template <int D, int QW, int KW>
 struct WideCfg {
-  static constexpr int TILE = 64 * D * 2;
+  static constexpr int NW = QW * KW;
+  static constexpr int U = D == 128 ? 2 / KW : 4 / KW;  // tiles of a wave and stage
+  static constexpr int KEYS = 32 * KW * U;
+  static constexpr int TILE = KEYS * D * 2;
   static constexpr int SMEM = 4 * TILE;
-  static constexpr int MASK_BYTES = 32 * QW * kMaskWords * 4;
+  static_assert(U >= 1 && (KW == 1 || KW / 2 * QW * 64 * (D / 32) * 64 <= SMEM), "the key waves' merge");
 };
 
-template <typename T, int D, bool NPOS, int QW>
+template <typename T, int D, bool NPOS, int QW, int KW>
 __device__ __forceinline__ void tree_wide_body(const TreeParams& p, char* smem, uint32_t* words, const TreeUnit& u) {
-  using C = WideCfg<D, QW>;
+  using C = WideCfg<D, QW, KW>;
   typedef T v4 __attribute__((ext_vector_type(4)));
-  constexpr int ND32 = D / 32;
+  constexpr int ND32 = D / 32, NW = C::NW;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qw = wave / KW, kw = wave - qw * KW;
   const int l32 = lane & 31, hh = lane >> 5;
-  const float n = *p.n_ptr;
-  const float c = p.scale * *p.b_ptr;
   const LoadLane lk(lane, wave, p.k.ss), lv(lane, wave, p.v.ss);
   const uint32_t lds0 = lds_addr(smem);
   const RowBase<D> rb(l32, hh);
   const TrBase<D> tb(lane);
-  const int nst = (u.kend - u.kbeg + 63) / 64;
+  const int nst = (u.kend - u.kbeg + C::KEYS - 1) / C::KEYS;
   auto issue = [&](int i) {
     const uint32_t dst = lds0 + (i & 1) * 2 * C::TILE;
-    tile_load_async<D, 64, QW>(u.kg, p.k.ss, u.kbeg + 64 * i, u.kend, dst, wave, lk);
-    tile_load_async<D, 64, QW>(u.vg, p.v.ss, u.kbeg + 64 * i, u.kend, dst + C::TILE, wave, lv);
+    tile_load_async<D, C::KEYS, NW>(u.kg, p.k.ss, u.kbeg + C::KEYS * i, u.kend, dst, wave, lk);
+    tile_load_async<D, C::KEYS, NW>(u.vg, p.v.ss, u.kbeg + C::KEYS * i, u.kend, dst + C::TILE, wave, lv);
   };
   if (nst > 0) issue(0);
+  const float n = *p.n_ptr;
+  const float c = p.scale * *p.b_ptr;
   RowGroup<T, D> st[1];
-  const int row = 32 * wave + l32;
+  const int row = 32 * qw + l32;
   st[0].init(p, u, row, hh);
   const bool reaches = nst > 0 && u.kend > u.base;
-  if (reaches) pack_mask(p, u, words, tid, QW * 64);
+  if (reaches) pack_mask(p, u, words, tid, NW * 64);
   const uint32_t* mrow =
       words + ((u.row0 + min(row, u.nrows - 1)) / u.G - u.row0 / u.G) * mask_stride(p.T);
-  const bool works = 32 * wave < u.nrows;
+  const bool works = 32 * qw < u.nrows;
   for (int i = 0; i < nst; ++i) {
     wait_vm<0>();     // this wave's share of stage i has landed
     __syncthreads();  // and everyone's; everyone is done with the other buffer
     if (i + 1 < nst) issue(i + 1);
     if (!works) continue;
-    const uint32_t buf = lds0 + (i & 1) * 2 * C::TILE;
+    const uint32_t buf = lds0 + (i & 1) * 2 * C::TILE + kw * BlockLayout<D>::BLOCK;
     const RowBase<D> kr = at_tile(rb, buf);
     const TrBase<D> vt = at_tile(tb, buf + C::TILE);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int key0 = u.kbeg + 64 * i + 32 * t;
+    for (int t = 0; t < C::U; ++t) {
+      const int key0 = u.kbeg + C::KEYS * i + 32 * (kw + KW * t);
       if (key0 >= u.kend) break;
       uint32_t win[1] = {0};
       if (u.masked(key0)) {
         win[0] = mask_window(mrow, key0 - u.base) >> (4 * hh);
-        tree_tile<T, D, NPOS, true, 1>(kr, vt, t, st, win, c, n);
+        tree_tile<T, D, NPOS, true, 1>(kr, vt, KW * t, st, win, c, n);
       } else {
-        tree_tile<T, D, NPOS, false, 1>(kr, vt, t, st, win, c, n);
+        tree_tile<T, D, NPOS, false, 1>(kr, vt, KW * t, st, win, c, n);
       }
     }
   }
-  const float l = pair_sum(st[0].l);
+  float m = st[0].m, l = st[0].l;
+  // the upper half of the key waves hands its (m, l, acc) to the lower, lane by
+  // lane through LDS, until one is left
+  if constexpr (KW > 1) {
+    f32x4_t* accs = reinterpret_cast<f32x4_t*>(smem);
+    float* ml = reinterpret_cast<float*>(words);
+#pragma unroll
+    for (int half = KW / 2; half >= 1; half /= 2) {
+      __syncthreads();  // the stages, or the last exchange, have been read
+      const int slot = qw * half + (kw - half);
+      if (works && kw >= half && kw < 2 * half) {
+        ml[(2 * slot) * 64 + lane] = m;
+        ml[(2 * slot + 1) * 64 + lane] = l;
+#pragma unroll
+        for (int j = 0; j < 4 * ND32; ++j) {
+          f32x4_t x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = st[0].acc[j / 4][4 * (j % 4) + e];
+          accs[(slot * 4 * ND32 + j) * 64 + lane] = x;
+        }
+      }
+      __syncthreads();
+      if (works && kw < half) {
+        const int from = qw * half + kw;
+        const float m2 = ml[(2 * from) * 64 + lane], l2 = ml[(2 * from + 1) * 64 + lane];
+        const float M = fmaxf(m, m2), ref = M == -INFINITY ? 0.f : M;
+        const float f1 = fast_exp2(m - ref), f2 = fast_exp2(m2 - ref);
+        m = M;
+        l = l * f1 + l2 * f2;
+#pragma unroll
+        for (int j = 0; j < 4 * ND32; ++j) {
+          const f32x4_t x = accs[(from * 4 * ND32 + j) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st[0].acc[j / 4][4 * (j % 4) + e] = st[0].acc[j / 4][4 * (j % 4) + e] * f1 + x[e] * f2;
+        }
+      }
+    }
+    if (kw > 0) return;
+  }
+  l = pair_sum(l);
   if (row >= u.nrows) return;
   const RowOut o(p, u, row);
   if (p.splits == 1) {
@@ -455,7 +528,7 @@ __device__ __forceinline__ void tree_wide_body(const TreeParams& p, char* smem, 
         *reinterpret_cast<v4*>(dst + 32 * db + 8 * g + 4 * hh) = x;
       }
     }
-    if (hh == 0 && p.m != nullptr) p.m[o.mrow] = st[0].m + log2f(l_safe);
+    if (hh == 0 && p.m != nullptr) p.m[o.mrow] = m + log2f(l_safe);
   } else {
     float* dst = p.ws_acc + o.rec * D;
 #pragma unroll
@@ -469,7 +542,7 @@ __device__ __forceinline__ void tree_wide_body(const TreeParams& p, char* smem, 
       }
     }
     if (hh == 0) {
-      p.ws_ml[2 * o.rec] = st[0].m;
+      p.ws_ml[2 * o.rec] = m;
       p.ws_ml[2 * o.rec + 1] = l;
     }
   }
@@ -483,51 +556,65 @@ __global__ __launch_bounds__(DecodeCfg<D>::NW * 64) void tree_stream_kernel(Tree
   __shared__ uint32_t words[32 * NQ * kMaskWords];
   const int block = folded_block();
   if (block >= nunits) return;
-  const TreeUnit u(p, block, 32 * NQ, 1, 32 * DecodeCfg<D>::NW);
+  const TreeUnit u(p, block, 32 * NQ, 1);
+  if (p.splits > 1 && u.kend <= u.kbeg) return;  // a shorter sequence: nothing to merge
   if (*p.n_ptr >= 0.f)
     tree_stream_body<T, D, true, NQ>(p, smem, words, u);
   else
     tree_stream_body<T, D, false, NQ>(p, smem, words, u);
 }
 
-template <typename T, int D, int QW>
-__global__ __launch_bounds__(QW * 64) void tree_wide_kernel(TreeParams p, int nunits, int nqb) {
-  __shared__ __attribute__((aligned(1024))) char smem[WideCfg<D, QW>::SMEM];
+template <typename T, int D, int QW, int KW>
+__global__ __launch_bounds__(QW* KW * 64) void tree_wide_kernel(TreeParams p, int nunits, int nqb) {
+  __shared__ __attribute__((aligned(1024))) char smem[WideCfg<D, QW, KW>::SMEM];
   __shared__ uint32_t words[32 * QW * kMaskWords];
   const int block = folded_block();
   if (block >= nunits) return;
-  const TreeUnit u(p, block, 32 * QW, nqb, 64);
+  const TreeUnit u(p, block, 32 * QW, nqb);
+  if (p.splits > 1 && u.kend <= u.kbeg) return;  // a shorter sequence: nothing to merge
   if (*p.n_ptr >= 0.f)
-    tree_wide_body<T, D, true, QW>(p, smem, words, u);
+    tree_wide_body<T, D, true, QW, KW>(p, smem, words, u);
   else
-    tree_wide_body<T, D, false, QW>(p, smem, words, u);
+    tree_wide_body<T, D, false, QW, KW>(p, smem, words, u);
 }
 
 // The splits' partials of a row in split order: out = sum_s acc_s 2^(m_s - M) /
-// sum_s l_s 2^(m_s - M).  D / 4 threads a row, four columns each; every load is
-// independent of the running state.
-template <typename T, int D>
+// sum_s l_s 2^(m_s - M).  D / 4 threads a row, four columns each, and SW such
+// groups that take every SW-th split and meet in LDS; every load is independent
+// of the running state.
+template <typename T, int D, int SW>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p, int nrows) {
   typedef T v4 __attribute__((ext_vector_type(4)));
-  constexpr int TPR = D / 4, RPB = 256 / TPR;
-  const int row = folded_block() * RPB + threadIdx.x / TPR, col = threadIdx.x % TPR * 4;
-  if (row >= nrows) return;
-  const int64_t rec0 = static_cast<int64_t>(row) * p.splits;
-  const float* ml = p.ws_ml + 2 * rec0;
-  float M = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, ml[2 * s]);
-  const float ref = M == -INFINITY ? 0.f : M;
-  float Ls = 0.f;
-  f32x4_t O = f32x4_t{};
-#pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    const float f = fast_exp2(ml[2 * s] - ref);
-    Ls += ml[2 * s + 1] * f;
-    O += *reinterpret_cast<const f32x4_t*>(p.ws_acc + (rec0 + s) * D + col) * f;
-  }
+  constexpr int TPR = D / 4, RPB = 256 / (TPR * SW);
+  static_assert(RPB >= 1, "a row's threads in one workgroup");
+  __shared__ f32x4_t part[SW > 1 ? 256 : 1];
+  const int tid = threadIdx.x, col = tid % TPR * 4, sw = tid / TPR % SW, in = tid / (TPR * SW);
+  const int row = min(folded_block() * RPB + in, nrows - 1);  // a row past the end repeats the last
   const int G = p.Hq / p.Hkv, R = G * p.T;
   const int bh = row / R, r = row - bh * R, node = r / G;
   const int b = bh / p.Hkv, h = (bh - b * p.Hkv) * G + r - node * G;
+  const int64_t L = clamped_length(p, b);
+  const int ns = static_cast<int>((L + p.split_keys - 1) / p.split_keys);  // the sequence's own splits
+  const int64_t rec0 = static_cast<int64_t>(row) * p.splits;
+  const float* ml = p.ws_ml + 2 * rec0;
+  float M = -INFINITY;
+#pragma unroll 4
+  for (int s = 0; s < ns; ++s) M = fmaxf(M, ml[2 * s]);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float Ls = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < ns; ++s) Ls += ml[2 * s + 1] * fast_exp2(ml[2 * s] - ref);
+  f32x4_t O = f32x4_t{};
+#pragma unroll 4
+  for (int s = sw; s < ns; s += SW)
+    O += *reinterpret_cast<const f32x4_t*>(p.ws_acc + (rec0 + s) * D + col) * fast_exp2(ml[2 * s] - ref);
+  if constexpr (SW > 1) {
+    part[tid] = O;
+    __syncthreads();
+    if (sw > 0) return;
+#pragma unroll
+    for (int w = 1; w < SW; ++w) O += part[tid + w * TPR];
+  }
   const float l_safe = Ls == 0.f ? 1.f : Ls;
   const float inv = 1.f / l_safe;
   v4 x;
@@ -540,6 +627,12 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p, int nrows
 
 namespace {
 
+template <typename T, int D, int SW>
+void launch_merge(const TreeParams& p, hipStream_t s) {
+  const int n = p.B * p.Hq * p.T, rpb = 1024 / (D * SW);
+  hipLaunchKernelGGL((tree_merge_kernel<T, D, SW>), folded_grid((n + rpb - 1) / rpb, 256), dim3(256), 0, s, p, n);
+}
+
 template <typename T, int D>
 hipError_t launch_tree_t(const TreeParams& p, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(p.Hq / p.Hkv) * p.T;
@@ -547,18 +640,19 @@ hipError_t launch_tree_t(const TreeParams& p, hipStream_t s) {
   const int nqb = static_cast<int>((rows + per - 1) / per);
   const int units = static_cast<int>(tree_units(p.B, p.Hq, p.Hkv, p.T) * p.splits);
   constexpr int ST = DecodeCfg<D>::NW * 64;
+  constexpr int WT = D == 128 ? 512 : 1024, KW = D == 128 ? 1 : 2;  // threads; key waves of 8 row groups
   if (per == 32)
     hipLaunchKernelGGL((tree_stream_kernel<T, D, 1>), folded_grid(units, ST), dim3(ST), 0, s, p, units);
   else if (per == 64)
     hipLaunchKernelGGL((tree_stream_kernel<T, D, 2>), folded_grid(units, ST), dim3(ST), 0, s, p, units);
   else if (per == 128)
-    hipLaunchKernelGGL((tree_wide_kernel<T, D, 4>), folded_grid(units, 256), dim3(256), 0, s, p, units, nqb);
+    hipLaunchKernelGGL((tree_wide_kernel<T, D, 4, 2 * KW>), folded_grid(units, WT), dim3(WT), 0, s, p, units, nqb);
   else
-    hipLaunchKernelGGL((tree_wide_kernel<T, D, 8>), folded_grid(units, 512), dim3(512), 0, s, p, units, nqb);
-  if (p.splits > 1) {
-    const int n = p.B * p.Hq * p.T, rpb = 1024 / D;
-    hipLaunchKernelGGL((tree_merge_kernel<T, D>), folded_grid((n + rpb - 1) / rpb, 256), dim3(256), 0, s, p, n);
-  }
+    hipLaunchKernelGGL((tree_wide_kernel<T, D, 8, KW>), folded_grid(units, WT), dim3(WT), 0, s, p, units, nqb);
+  if (p.splits > 8)
+    launch_merge<T, D, 4>(p, s);
+  else if (p.splits > 1)
+    launch_merge<T, D, 1>(p, s);
   return hipGetLastError();
 }
 

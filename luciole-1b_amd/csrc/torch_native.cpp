@@ -49,6 +49,7 @@ struct CacheAbi {  // include/ssa_cache_ops.h
   decltype(&ssa_tree_attention) tree;
   decltype(&ssa_tree_workspace_bytes) tree_bytes;
   decltype(&ssa_key_weights) key_weights;
+  decltype(&ssa_key_weights_workspace_bytes) key_weights_bytes;
   decltype(&ssa_cache_evict) evict;
   decltype(&ssa_cache_accept) accept;
 };
@@ -561,10 +562,13 @@ PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int32_t status;
   {
     pybind11::gil_scoped_release unlocked;
+    const int64_t ws_bytes = cache_abi.key_weights_bytes(i32(c.B), i32(Hq), i32(c.Hkv), i32(c.cap), i32(T));
+    at::Tensor ws;
+    if (ws_bytes > 0) ws = bytes(ws_bytes, *q);
     const ssa_key_weights_args f{qv, view(*k), static_cast<const float*>(m->data_ptr()),
                                  static_cast<float*>(w->data_ptr()), w->stride(0), w->stride(1), int_data(*lens), np,
                                  bp, i32(c.B), i32(Hq), i32(c.Hkv), i32(c.cap), i32(c.D), c.dtype, i32(T),
-                                 static_cast<float>(scale)};
+                                 static_cast<float>(scale), ws.defined() ? ws.data_ptr() : nullptr};
     status = cache_abi.key_weights(&f, in.stream);
   }
   if (status != 0) return PyLong_FromLong(status);
