@@ -36,15 +36,25 @@ __device__ __forceinline__ int clamped_len(const int* lens, int b, int cap) {
   return L < 0 ? 0 : (L > cap ? cap : L);
 }
 
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  // within rows of 16 lanes, then each row's last lane into the next row(s)
+#define SSA_DPP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0u, x, ctrl, rows, 0xf, false)
+  SSA_DPP(0x111, 0xf);  // row_shr:1
+  SSA_DPP(0x112, 0xf);  // row_shr:2
+  SSA_DPP(0x114, 0xf);  // row_shr:4
+  SSA_DPP(0x118, 0xf);  // row_shr:8
+  SSA_DPP(0x142, 0xa);  // row_bcast:15
+  SSA_DPP(0x143, 0xc);  // row_bcast:31
+#undef SSA_DPP
+  return x;
+}
+
 // Inclusive sum over the workgroup's threads (kSelect of them); `waves` holds
 // one value per wave.  Two barriers.
 __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* waves, int tid, uint32_t& total) {
   const int lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint32_t y = __shfl_up(x, off, 64);
-    if (lane >= off) x += y;
-  }
+  x = wave_scan(x);
   __syncthreads();  // the last scan's values have been read
   if (lane == 63) waves[wave] = x;
   __syncthreads();
@@ -61,15 +71,17 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* waves, int 
 
 }  // namespace
 
-// E rows a thread at a time, four consecutive ones per 4096: a cache of up to
-// 1024 E rows is read once and stays in registers for every pass, a longer one
-// is read in such stretches by each of the four.
+// A wave takes 64 E consecutive rows, four consecutive ones a lane at a time, a
+// workgroup 1024 E: a cache of up to that many rows is read once and its keys
+// stay in registers for every pass, a longer one is read by each.  Rows that
+// stay in any case rank above every weight and rows past the length below or
+// with the lowest, where the lower row wins.
 template <int E>
 __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams p, int nblocks) {
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t waves[kSelect / 64];
   __shared__ uint32_t found[2];  // digit, rows above it
-  const int tid = threadIdx.x, block = folded_block();
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, block = folded_block();
   if (block >= nblocks) return;
   const int b = block / p.Hkv, h = block - b * p.Hkv;
   const int L = clamped_len(p.seqlens, b, p.cap);
@@ -83,98 +95,112 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams p, in
     for (int i = tid; i < p.keep; i += kSelect) kept[i] = i < L ? i : -1;
     return;
   }
-  for (int i = p.keep + tid; i < p.cap; i += kSelect) w_out[i] = 0.f;
   constexpr int STRETCH = kSelect * E;
-  float v[E];
+  const int mine = wave * 64 * E + 4 * lane;  // the lane's first row of a stretch; then every 256th
+  const int lo = p.sinks, hi = L - p.recent;  // rows [lo, hi) are chosen from
+  uint32_t key[E];
   auto load = [&](int r0) {
 #pragma unroll
     for (int j = 0; j < E / 4; ++j) {
-      const int i = r0 + 4 * kSelect * j + 4 * tid;
+      const int i = r0 + mine + 256 * j;
+      f32x4_u x = {0.f, 0.f, 0.f, 0.f};
       if (i + 3 < L) {
-        const f32x4_u x = *reinterpret_cast<const f32x4_u*>(w + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * j + e] = x[e];
+        x = *reinterpret_cast<const f32x4_u*>(w + i);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * j + e] = i + e < L ? w[i + e] : 0.f;
+        for (int e = 0; e < 4; ++e)
+          if (i + e < L) x[e] = w[i + e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t k = order_bits(x[e]);
+        key[4 * j + e] = i + e >= L ? 0u : (i + e < lo || i + e >= hi) ? 0xffffffffu : k;
       }
     }
   };
   const bool once = L <= STRETCH;
   if (once) load(0);
-  // rows [lo, hi) are chosen from; sinks + recent <= keep < L, so lo < hi
-  const int lo = p.sinks, hi = L - p.recent;
-  uint32_t need = p.keep - p.sinks - p.recent;  // of them stay, fewer than there are
+  for (int i = p.keep + tid; i < p.cap; i += kSelect) w_out[i] = 0.f;
+  uint32_t need = p.keep;  // rows that stay, of those that share the prefix
   uint32_t prefix = 0;
-  const bool choose = need > 0;
-  if (choose) {
-    constexpr int kShift[3] = {20, 10, 0}, kWidth[3] = {12, 10, 10};
+  constexpr int kShift[3] = {20, 10, 0}, kWidth[3] = {12, 10, 10};
 #pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-      const int bins = 1 << kWidth[pass];
-      for (int i = tid; i < bins; i += kSelect) hist[i] = 0;
-      __syncthreads();
-      for (int r0 = 0; r0 < L; r0 += STRETCH) {
-        if (!once) load(r0);
+  for (int pass = 0; pass < 3; ++pass) {
+    const int bins = 1 << kWidth[pass];
+    for (int i = tid; i < bins; i += kSelect) hist[i] = 0;
+    __syncthreads();
+    for (int r0 = 0; r0 < L; r0 += STRETCH) {
+      if (!once) load(r0);
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const int i = r0 + 4 * kSelect * (j / 4) + 4 * tid + j % 4;
-          const uint32_t key = order_bits(v[j]);
-          if (i >= lo && i < hi && (pass == 0 || (key >> (kShift[pass] + kWidth[pass])) == prefix))
-            atomicAdd(&hist[(key >> kShift[pass]) & (bins - 1)], 1u);
-        }
-      }
-      __syncthreads();
-      // bins from the top: thread i takes `per` bins downwards from the i-th group
-      const int per = bins / kSelect;
-      uint32_t mine = 0;
-      for (int x = 0; x < per; ++x) mine += hist[bins - 1 - per * tid - x];
-      uint32_t total;
-      const uint32_t upto = block_scan(mine, waves, tid, total);
-      uint32_t above = upto - mine;
-      if (above < need && upto >= need) {
-        int bin = bins - 1 - per * tid;
-        while (above + hist[bin] < need) above += hist[bin--];
-        found[0] = bin;
-        found[1] = above;
-      }
-      __syncthreads();
-      prefix = (prefix << kWidth[pass]) | found[0];
-      need -= found[1];
+      for (int j = 0; j < E; ++j)
+        if (pass == 0 || (key[j] >> (kShift[pass] + kWidth[pass])) == prefix)
+          atomicAdd(&hist[(key[j] >> kShift[pass]) & (bins - 1)], 1u);
     }
+    __syncthreads();
+    // bins from the top: thread i takes `per` bins downwards from the i-th group
+    const int per = bins / kSelect;
+    uint32_t sum = 0;
+    for (int x = 0; x < per; ++x) sum += hist[bins - 1 - per * tid - x];
+    uint32_t total;
+    const uint32_t upto = block_scan(sum, waves, tid, total);
+    uint32_t above = upto - sum;
+    if (above < need && upto >= need) {
+      int bin = bins - 1 - per * tid;
+      while (above + hist[bin] < need) above += hist[bin--];
+      found[0] = bin;
+      found[1] = above;
+    }
+    __syncthreads();
+    prefix = (prefix << kWidth[pass]) | found[0];
+    need -= found[1];
   }
   const uint32_t ties = need;  // rows at the threshold that stay, the lowest first
-  uint32_t above0 = 0, at0 = 0;  // rows before this stretch that surely stay; at the threshold
+  uint32_t above0 = 0, at0 = 0;  // rows before this stretch above the threshold; at it
   for (int r0 = 0; r0 < L; r0 += STRETCH) {
     if (!once) load(r0);
+    // the wave's counts: above in the low half, at the threshold in the high
+    uint32_t up = 0, eq = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      up += key[j] > prefix;
+      eq += key[j] == prefix;
+    }
+    // a wave's 64 E rows are at most 2^11, a workgroup's at most 2^15: no carry
+    uint32_t total, before_waves = 0;
+    {
+      const uint32_t sum = wave_scan(up | (eq << 16));
+      __syncthreads();
+      if (lane == 63) waves[wave] = sum;
+      __syncthreads();
+      total = 0;
+#pragma unroll
+      for (int x = 0; x < kSelect / 64; ++x) {
+        before_waves += x < wave ? waves[x] : 0;
+        total += waves[x];
+      }
+    }
 #pragma unroll
     for (int j = 0; j < E / 4; ++j) {
-      const int first = r0 + 4 * kSelect * j;
-      if (first >= L) break;
-      uint32_t up[4], eq[4], count = 0;
+      uint32_t count = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) count += (key[4 * j + e] > prefix) + ((key[4 * j + e] == prefix) << 16);
+      const uint32_t upto = wave_scan(count);
+      uint32_t before = before_waves + upto - count;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int i = first + 4 * tid + e;
-        const uint32_t key = order_bits(v[4 * j + e]);
-        const bool inside = i >= lo && i < hi;
-        up[e] = i < L && (!inside || (choose && key > prefix));
-        eq[e] = inside && choose && key == prefix;
-        count += up[e] + (eq[e] << 16);
-      }
-      uint32_t total;
-      uint32_t before = block_scan(count, waves, tid, total) - count;  // both at most 2^12: no carry
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
+        const bool over = key[4 * j + e] > prefix, even = key[4 * j + e] == prefix;
         const uint32_t at = at0 + (before >> 16), place = above0 + (before & 0xffffu) + (at < ties ? at : ties);
-        if (up[e] || (eq[e] && at < ties)) {
-          kept[place] = first + 4 * tid + e;
-          w_out[place] = v[4 * j + e];
+        if (over || (even && at < ties)) {
+          const int i = r0 + mine + 256 * j + e;
+          kept[place] = i;
+          w_out[place] = w[i];
         }
-        before += up[e] + (eq[e] << 16);
+        before += over + (even << 16);
       }
-      above0 += total & 0xffffu;
-      at0 += total >> 16;
+      before_waves += __builtin_amdgcn_readlane(upto, 63);
     }
+    above0 += total & 0xffffu;
+    at0 += total >> 16;
   }
 }
 
@@ -284,9 +310,15 @@ hipError_t launch_evict(const EvictParams& p, hipStream_t s) {
     hipLaunchKernelGGL(evict_select_kernel<16>, grid, dim3(kSelect), 0, s, p, heads);
   else
     hipLaunchKernelGGL(evict_select_kernel<32>, grid, dim3(kSelect), 0, s, p, heads);
-  const int slices = p.D / 8 / 4;  // 64-byte slices
-  const int blocks = heads * 2 * slices;
-  hipLaunchKernelGGL((evict_move_kernel<4>), folded_grid(blocks, 1024), dim3(1024), 0, s, p, slices, blocks);
+  const auto move = [&](auto kernel, int sp) {
+    const int slices = p.D / 8 / sp;
+    const int blocks = heads * 2 * slices;
+    hipLaunchKernelGGL(kernel, folded_grid(blocks, 1024), dim3(1024), 0, s, p, slices, blocks);
+  };
+  if (heads * 2 * (p.D / 32) < 256)
+    move(evict_move_kernel<2>, 2);
+  else
+    move(evict_move_kernel<4>, 4);
   return hipGetLastError();
 }
 

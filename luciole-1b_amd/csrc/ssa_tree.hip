@@ -17,7 +17,7 @@
 //   * up to 64 rows (tree_stream_kernel): the cache's stream is the bound; each
 //     wave streams its own tiles of 32 keys through a private LDS ring, for one
 //     or two groups of 32 rows at once, and the waves merge at the end;
-//   * more (tree_wide_kernel): the transform (one log2 and one exp2 a pair) is
+//   * more (tree_kernel): the transform (one log2 and one exp2 a pair) is
 //     the bound; QW groups of 32 rows by KW key waves share each stage of keys,
 //     and the key waves merge at the end.
 // The keys are split over workgroups in ranges of one length for all sequences
@@ -25,17 +25,17 @@
 // result does not depend on the others); partials (m, l, acc) meet in split
 // order in tree_merge_kernel.
 //
-// The running maximum is moved only when a lane's sum of a tile passes a bound
-// with the old one (kTreeSum): the rescaling of acc and the tile's maximum are
-// then rare, a quarter of the vector work.
+// The reference m of a row's exponents is its running maximum only loosely: it
+// starts at 0 where that suits the first scores and moves to the maximum when a
+// lane's sum of a tile passes a bound (kTreeSum), so that the rescaling of acc
+// and the tile's maximum, a quarter of the vector work, are rare.
 //
 // The mask is packed to one bit per node when a workgroup's keys reach the
 // tree's rows; tiles before them do no mask work.
 #include "ssa_cache_ops.hpp"
 #include "ssa_common.hpp"
 #include "ssa_launch.hpp"
-#include "ssa_plan.hpp"
-#include "ssa_tile.hpp"
+#include "ssa_row_tile.hpp"
 
 namespace ssa {
 
@@ -58,6 +58,7 @@ struct TreeUnit {
   int G, base, kbeg, kend, ntile;
   const char* kg;
   const char* vg;
+  float n, c;  // t = n sign(s) log2(1 + c |s|)
   __device__ __forceinline__ TreeUnit(const TreeParams& p, int block, int per, int nqb) {
     int u = block;
     // the splits' first ranges of all sequences, then the second ones ...: the
@@ -69,10 +70,14 @@ struct TreeUnit {
     u -= qb * nbh;
     b = u / p.Hkv;
     hk = u - b * p.Hkv;
+    // the three scalars a workgroup waits for, on their way together
+    const int held = load_table_entry(p.seqlens, b);
+    n = __int_as_float(load_table_entry(reinterpret_cast<const int*>(p.n_ptr), 0));
+    c = p.scale * __int_as_float(load_table_entry(reinterpret_cast<const int*>(p.b_ptr), 0));
     G = p.Hq / p.Hkv;
     row0 = qb * per;
     nrows = min(per, G * p.T - row0);
-    const int L = clamped_length(p, b);
+    const int L = held < 0 ? 0 : (held > p.cap ? p.cap : held);
     base = L - p.T;
     const int64_t beg = static_cast<int64_t>(split) * p.split_keys;
     kbeg = beg < L ? static_cast<int>(beg) : L;
@@ -107,6 +112,7 @@ __device__ __forceinline__ void pack_mask(const TreeParams& p, const TreeUnit& u
 
 // Keys key0 .. key0 + 31 that a node sees, as bits; j0 = key0 - base < T.
 __device__ __forceinline__ uint32_t mask_window(const uint32_t* row, int j0) {
+  if (j0 <= -32) return 0xffffffffu;
   if (j0 < 0) return (row[0] << -j0) | ((1u << -j0) - 1u);
   return __builtin_amdgcn_alignbit(row[(j0 >> 5) + 1], row[j0 >> 5], j0 & 31);
 }
@@ -132,12 +138,6 @@ struct RowGroup {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ bool not_finite(uint32_t two) {
-  constexpr uint32_t E = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
-  return (two & E) == E || (two & (E << 16)) == (E << 16);
-}
-
 // All ones where bit `i` of win is set, else 0.
 __device__ __forceinline__ uint32_t seen_mask(uint32_t win, int i) {
   return static_cast<uint32_t>(static_cast<int32_t>(win << (31 - i)) >> 31);
@@ -145,138 +145,140 @@ __device__ __forceinline__ uint32_t seen_mask(uint32_t win, int i) {
 // Bit of accumulator entry r in a window shifted by 4 hh (crow()).
 __device__ __forceinline__ constexpr int bit_of(int r) { return 8 * (r >> 2) + (r & 3); }
 
-// What the infinities and NaN of a tile of V add to the rows that see them:
-// kind 0 / 1 / 2 counts the +inf / -inf / NaN that each row sees in each
-// column, by a product with the rows' 0 / 1 masks.
-template <typename T, int D, int NQ>
-__device__ void add_not_finite(const TrBase<D>& vt, int blk, RowGroup<T, D> (&st)[NQ], const uint32_t (&win)[NQ]) {
-  typedef typename Vec8<T>::type v8;
-  typedef T v4 __attribute__((ext_vector_type(4)));
+// The sign bit of each half of a word that holds an infinity or NaN: adding one
+// to an exponent of all ones carries into it.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t two) {
+  constexpr uint32_t E = __is_same(T, __bf16) ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t ONE = __is_same(T, __bf16) ? 0x00800080u : 0x04000400u;
+  return ((two & E) + ONE) & 0x80008000u;
+}
+
+// A masked row's p is 0, and 0 times an infinity or NaN is not: such values of a
+// block of V (32 rows at vat) become 0 in LDS, and `bad` there tells
+// add_not_finite() to add them where they are seen.  Waves that share the block
+// write the same.
+template <typename T, int D>
+__device__ __forceinline__ void clear_not_finite(uint32_t vat, int lane, int* bad) {
 #pragma unroll 1
-  for (int kind = 0; kind < 3; ++kind) {
-    const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
+  for (int i = 0; i < RowTile<D>::PIECES; ++i) {
+    auto at = (__attribute__((address_space(3))) u32x4*)(uintptr_t)(vat + RowTile<D>::off(i) + lane * 16);
+    u32x4 w = *at;
+    uint32_t any = 0;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db) {
-      v8 hit[2];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const v4 lo = tile_read_tr<D, v4>(vt, blk, ks, 0, db), hi = tile_read_tr<D, v4>(vt, blk, ks, 1, db);
-        const v8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float v = static_cast<float>(vf[e]);
-          const bool is = kind == 0 ? v == INFINITY : kind == 1 ? v == -INFINITY : v != v;
-          hit[ks][e] = static_cast<T>(is ? 1.f : 0.f);
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < NQ; ++g) {
-        v8 seen[2];
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          seen[r >> 3][r & 7] = static_cast<T>(__uint_as_float(seen_mask(win[g], bit_of(r)) & 0x3f800000u));
-        f32x16 count = f32x16{};
-        count = mfma32(hit[0], seen[0], count);
-        count = mfma32(hit[1], seen[1], count);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[g].acc[db][r] += count[r] > 0.f ? add : 0.f;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t f = not_finite<T>(w[e]);
+      any |= f;
+      w[e] &= ~(f | (f - (f >> 15)));
+    }
+    if (any) {
+      *at = w;
+      *bad = 1;
     }
   }
 }
 
-// One tile of 32 keys for NQ groups of 32 rows: scores, transform, softmax
-// update and the product with V.  win[g]: the keys that the lane's row of group
-// g sees, shifted by 4 hh (MASKED).
-template <typename T, int D, bool NPOS, bool MASKED, int NQ>
-__device__ __forceinline__ void tree_tile(const RowBase<D>& kr, const TrBase<D>& vt, int blk, RowGroup<T, D> (&st)[NQ],
-                                          const uint32_t (&win)[NQ], float c, float n) {
+// One tile of 32 keys (blocks at kat and vat) for the wave's 32 rows: scores,
+// transform, softmax update and the product with V.  MASKED: win holds the keys
+// that the lane's row sees, shifted by 4 hh.
+template <typename T, int D, bool NPOS, bool MASKED>
+__device__ __forceinline__ void tree_tile(const RowTileK<D>& rk, const RowTileV<D>& rv, uint32_t kat, uint32_t vat,
+                                          RowGroup<T, D>& st, uint32_t win, float c, float n) {
   typedef typename Vec8<T>::type v8;
   typedef T v4 __attribute__((ext_vector_type(4)));
   constexpr int ND16 = D / 16, ND32 = D / 32;
   constexpr uint32_t kOut = NPOS ? 0xff800000u : 0x7f800000u;  // the score of the lowest t: -inf or +inf
-  f32x16 s[NQ];
+  f32x16 s = f32x16{};
 #pragma unroll
-  for (int g = 0; g < NQ; ++g) s[g] = f32x16{};
+  for (int ds = 0; ds < ND16; ++ds) s = mfma32(rk.template read<v8>(kat, ds), st.q[ds], s);
+  v8 pb[2];
+  bool done = false;
+  if constexpr (!MASKED) {
+    // a row that has seen nothing yet starts from 0: then its sum has to be
+    // large enough as well
+    const bool fresh = st.m == -INFINITY;
+    const float ref = fresh ? 0.f : st.m;
+    float sum = 0.f;
 #pragma unroll
-  for (int ds = 0; ds < ND16; ++ds) {
-    const v8 kf = tile_read_row<D, v8>(kr, blk, ds);
-#pragma unroll
-    for (int g = 0; g < NQ; ++g) s[g] = mfma32(kf, st[g].q[ds], s[g]);
-  }
-  v8 pb[NQ][2];
-#pragma unroll
-  for (int g = 0; g < NQ; ++g) {
-    if constexpr (!MASKED) {
-      float sum = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float x = s[g][r];
-        const float pv = fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -st[g].m));
-        sum += pv;
-        pb[g][r >> 3][r & 7] = static_cast<T>(pv);
-      }
-      // m = -inf (nothing seen yet) gives an infinite or NaN sum
-      if (__builtin_expect(__all(sum <= kTreeSum), 1)) {
-        st[g].l += sum;
-        continue;
-      }
+    for (int r = 0; r < 16; ++r) {
+      const float x = s[r];
+      const float pv = fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -ref));
+      sum += pv;
+      pb[r >> 3][r & 7] = static_cast<T>(pv);
     }
+    done = __all(sum <= kTreeSum && (!fresh || sum >= 1.f));
+    if (done) {
+      st.m = ref;
+      st.l += sum;
+    }
+  }
+  if (__builtin_expect(!done, MASKED)) {
     float z = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
+      float x = s[r];
+      pin(x);  // nothing of this branch is computed before it
       if constexpr (MASKED) {
-        const uint32_t in = seen_mask(win[g], bit_of(r));
-        s[g][r] = __uint_as_float((__float_as_uint(s[g][r]) & in) | (kOut & ~in));
+        const uint32_t in = seen_mask(win, bit_of(r));
+        x = __uint_as_float((__float_as_uint(x) & in) | (kOut & ~in));
       }
-      z = fmaxf(z, NPOS ? s[g][r] : -s[g][r]);
+      s[r] = x;
+      z = fmaxf(z, NPOS ? x : -x);
     }
     z = pair_max(z);
     const float top = NPOS ? z : -z;
     const float tmax = z == -INFINITY ? -INFINITY : n * copysignf(fast_log2(fmaf(c, fabsf(top), 1.f)), top);
-    const float mnew = fmaxf(st[g].m, tmax);
-    const float alpha = fast_exp2(mnew == -INFINITY ? 0.f : st[g].m - mnew);
-    st[g].m = mnew;
+    const float mnew = fmaxf(st.m, tmax);
+    const float alpha = fast_exp2(mnew == -INFINITY ? 0.f : st.m - mnew);
+    st.m = mnew;
 #pragma unroll
-    for (int d = 0; d < ND32; ++d) st[g].acc[d] *= alpha;
-    float l = st[g].l * alpha;
+    for (int d = 0; d < ND32; ++d) st.acc[d] *= alpha;
+    float l = st.l * alpha;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float x = s[g][r];
+      const float x = s[r];
       float pv = fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -mnew));
-      if constexpr (MASKED) pv = __uint_as_float(__float_as_uint(pv) & seen_mask(win[g], bit_of(r)));
+      if constexpr (MASKED) pv = __uint_as_float(__float_as_uint(pv) & seen_mask(win, bit_of(r)));
       l += pv;
-      pb[g][r >> 3][r & 7] = static_cast<T>(pv);
+      pb[r >> 3][r & 7] = static_cast<T>(pv);
     }
-    st[g].l = l;
+    st.l = l;
   }
-  bool bad = false;
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
     for (int db = 0; db < ND32; ++db) {
-      const v4 lo = tile_read_tr<D, v4>(vt, blk, ks, 0, db), hi = tile_read_tr<D, v4>(vt, blk, ks, 1, db);
-      v8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      if constexpr (MASKED) {
-        // a masked row's p is 0, and 0 times an infinity or NaN is not: such
-        // values leave the product here and join below where they are seen
-        const u32x4 w = __builtin_bit_cast(u32x4, vf);
-        const int b = int(not_finite<T>(w[0])) | int(not_finite<T>(w[1])) | int(not_finite<T>(w[2])) | int(not_finite<T>(w[3]));
-        if (__builtin_expect(__any(b), 0)) {
-          bad = true;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float v = static_cast<float>(vf[e]);
-            if (!(fabsf(v) < INFINITY)) vf[e] = static_cast<T>(0.f);
-          }
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < NQ; ++g) st[g].acc[db] = mfma32(vf, pb[g][ks], st[g].acc[db]);
+      const v4 lo = rv.template read<v4>(vat, ks, 0, db), hi = rv.template read<v4>(vat, ks, 1, db);
+      st.acc[db] = mfma32(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pb[ks], st.acc[db]);
     }
   }
-  if constexpr (MASKED) {
-    if (__builtin_expect(bad, 0)) add_not_finite<T, D, NQ>(vt, blk, st, win);
+}
+
+// The infinities and NaN that clear_not_finite() took out of the tree's rows of V, added
+// to the rows that see them: the wave's tiles from key0 on, every `step` keys.
+template <typename T, int D>
+__device__ __forceinline__ void add_not_finite(const TreeParams& p, const TreeUnit& u, const uint32_t* mrow, int key0,
+                                               int step, int hh, f32x16* acc) {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+#pragma unroll 1
+  for (int k0 = key0; k0 < u.kend; k0 += step) {
+    if (!u.masked(k0)) continue;
+    const uint32_t win = mask_window(mrow, k0 - u.base);
+#pragma unroll 1
+    for (int k = 0; k < 32; ++k) {
+      if (k0 + k >= u.kend) break;
+      const bool seen = win >> k & 1;
+      const T* row = reinterpret_cast<const T*>(u.vg) + (k0 + k) * p.v.ss + 4 * hh;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) {
+        const v4 x = *reinterpret_cast<const v4*>(row + 8 * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = static_cast<float>(x[e]);
+          acc[j / 4][4 * (j % 4) + e] += seen && !(fabsf(v) < INFINITY) ? v : 0.f;
+        }
+      }
+    }
   }
 }
 
@@ -293,223 +295,151 @@ struct RowOut {
   }
 };
 
-// ------------------------------------------------------------ up to 64 rows
-template <int D, int NQ>
-struct StreamCfg : DecodeCfg<D> {
-  using C = DecodeCfg<D>;
-  static constexpr int MASK_BYTES = 32 * NQ * kMaskWords * 4;
-};
-
-template <typename T, int D, bool NPOS, int NQ>
-__device__ __forceinline__ void tree_stream_body(const TreeParams& p, char* smem, uint32_t* words, const TreeUnit& u) {
-  using C = DecodeCfg<D>;
-  constexpr int NW = C::NW, NB = C::NB, ND32 = D / 32;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l32 = lane & 31, hh = lane >> 5;
-  const float n = *p.n_ptr;
-  const float c = p.scale * *p.b_ptr;
-  const int ntw = u.ntile > wave ? (u.ntile - wave + NW - 1) / NW : 0;  // tiles of this wave
-
-  const LoadLane lk0(lane, 0, p.k.ss), lk1(lane, 1, p.k.ss), lv0(lane, 0, p.v.ss), lv1(lane, 1, p.v.ss);
-  const uint32_t ring = lds_addr(smem) + wave * NB * C::TB;
-  const RowBase<D> rb(l32, hh);
-  const TrBase<D> tb(lane);
-  // past the wave's last tile the rows clamp to kend - 1 (loads into a free
-  // buffer, never read), so that one wait count fits every iteration
-  auto issue = [&](int i) {
-    const int row0 = u.kbeg + 32 * (wave + NW * i);
-    const uint32_t dst = ring + (i % NB) * C::TB;
-    block_load_wave<D>(u.kg, p.k.ss, row0, u.kend, dst, lk0, lk1);
-    block_load_wave<D>(u.vg, p.v.ss, row0, u.kend, dst + C::BLOCK, lv0, lv1);
-  };
-  if (ntw > 0) {
-#pragma unroll
-    for (int i = 0; i < NB - 1; ++i) issue(i);
-  }
-  RowGroup<T, D> st[NQ];
-#pragma unroll
-  for (int g = 0; g < NQ; ++g) st[g].init(p, u, 32 * g + l32, hh);
-  const bool reaches = u.kend > u.kbeg && u.kend > u.base;
-  if (reaches) pack_mask(p, u, words, tid, NW * 64);
-  __syncthreads();
-  if (ntw > 0) {
-    const int W = mask_stride(p.T), n0 = u.row0 / u.G;
-    const uint32_t* mrow[NQ];
-#pragma unroll
-    for (int g = 0; g < NQ; ++g) mrow[g] = words + ((u.row0 + min(32 * g + l32, u.nrows - 1)) / u.G - n0) * W;
-    for (int i = 0; i < ntw; ++i) {
-      wait_lgkm<0>();  // reads of tile i - 1, whose buffer the next issue overwrites
-      issue(i + NB - 1);
-      wait_vm<(NB - 1) * C::LPT>();  // tile i has landed
-      const uint32_t buf = ring + (i % NB) * C::TB;
-      const RowBase<D> kr = at_tile(rb, buf);
-      const TrBase<D> vt = at_tile(tb, buf + C::BLOCK);
-      const int key0 = u.kbeg + 32 * (wave + NW * i);
-      uint32_t win[NQ] = {};
-      if (u.masked(key0)) {
-#pragma unroll
-        for (int g = 0; g < NQ; ++g) win[g] = mask_window(mrow[g], key0 - u.base) >> (4 * hh);
-        tree_tile<T, D, NPOS, true, NQ>(kr, vt, 0, st, win, c, n);
-      } else {
-        tree_tile<T, D, NPOS, false, NQ>(kr, vt, 0, st, win, c, n);
-      }
-    }
-    wait_vm<0>();  // the trailing prefetches land before the ring is reused
-  }
-
-  // Merge the waves: (m, l) per row and acc[row][d] through LDS, then one
-  // thread per (row, d) combines them in wave order.
-  float* ml = reinterpret_cast<float*>(smem);                  // [NW][2][32]
-  float* accs = reinterpret_cast<float*>(smem + C::ML_BYTES);  // [NW][32][ACC_LD]
-#pragma unroll
-  for (int g = 0; g < NQ; ++g) {
-    const float l_tot = pair_sum(st[g].l);
-    __syncthreads();
-    if (hh == 0) {
-      ml[(wave * 2 + 0) * 32 + l32] = st[g].m;
-      ml[(wave * 2 + 1) * 32 + l32] = l_tot;
-    }
-#pragma unroll
-    for (int db = 0; db < ND32; ++db) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) accs[(wave * 32 + l32) * C::ACC_LD + db * 32 + crow(r, hh)] = st[g].acc[db][r];
-    }
-    __syncthreads();
-    const int rows = min(32, u.nrows - 32 * g);
-    for (int e = tid; e < rows * D; e += NW * 64) {
-      const int q = e / D, d = e - q * D;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[(w * 2) * 32 + q]);
-      float Ls = 0.f, O = 0.f;
-      if (M != -INFINITY) {
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const float sc = fast_exp2(ml[(w * 2) * 32 + q] - M);
-          // a wave that saw no key of this row has m = -inf, l = 0, acc = 0
-          Ls += ml[(w * 2 + 1) * 32 + q] * sc;
-          O += accs[(w * 32 + q) * C::ACC_LD + d] * sc;
-        }
-      }
-      const RowOut o(p, u, 32 * g + q);
-      if (p.splits == 1) {
-        const float l_safe = Ls == 0.f ? 1.f : Ls;
-        static_cast<T*>(const_cast<void*>(p.o.ptr))[o.off + d] = static_cast<T>(O * (1.f / l_safe));
-        if (d == 0 && p.m != nullptr) p.m[o.mrow] = M + log2f(l_safe);
-      } else {
-        p.ws_acc[o.rec * D + d] = O;
-        if (d == 0) {
-          p.ws_ml[2 * o.rec] = M;
-          p.ws_ml[2 * o.rec + 1] = Ls;
-        }
-      }
-    }
-  }
-}
-
-// ------------------------------------------------------------ more than 64 rows
 // Two stages of 32 KW U keys, a K tile and a V tile each; wave (qw, kw) takes
 // the stage's key tiles kw, kw + KW, ...
 template <int D, int QW, int KW>
-struct WideCfg {
+struct TreeCfg {
   static constexpr int NW = QW * KW;
-  static constexpr int U = D == 128 ? 2 / KW : 4 / KW;  // tiles of a wave and stage
-  static constexpr int KEYS = 32 * KW * U;
-  static constexpr int TILE = KEYS * D * 2;
-  static constexpr int SMEM = 4 * TILE;
-  static_assert(U >= 1 && (KW == 1 || KW / 2 * QW * 64 * (D / 32) * 64 <= SMEM), "the key waves' merge");
+  static constexpr int U = KW == 1 ? 2 : 1;  // tiles of a wave and stage
+  static constexpr int BLOCKS = KW * U;
+  static constexpr int KEYS = 32 * BLOCKS;
+  static constexpr int TILE = BLOCKS * RowTile<D>::BLOCK;
+  // the key waves' exchange: each hands the others their shares of its acc
+  static constexpr int J = D / 8;                    // float4 of a lane's acc
+  static constexpr int JB = J > KW ? J / KW : 1;     // of a wave's share
+  static constexpr int MERGE = KW == 1 ? 0 : QW * J * (KW - 1) * 1024;
+  static constexpr int SMEM = 4 * TILE > MERGE ? 4 * TILE : MERGE;
+  static constexpr int WORDS = 32 * QW * kMaskWords > 128 * NW ? 32 * QW * kMaskWords : 128 * NW;
 };
 
 template <typename T, int D, bool NPOS, int QW, int KW>
-__device__ __forceinline__ void tree_wide_body(const TreeParams& p, char* smem, uint32_t* words, const TreeUnit& u) {
-  using C = WideCfg<D, QW, KW>;
+__device__ __forceinline__ void tree_body(const TreeParams& p, char* smem, uint32_t* words, int* bad,
+                                          const TreeUnit& u) {
+  using C = TreeCfg<D, QW, KW>;
   typedef T v4 __attribute__((ext_vector_type(4)));
-  constexpr int ND32 = D / 32, NW = C::NW;
+  constexpr int NW = C::NW;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qw = wave / KW, kw = wave - qw * KW;
   const int l32 = lane & 31, hh = lane >> 5;
-  const LoadLane lk(lane, wave, p.k.ss), lv(lane, wave, p.v.ss);
+  const RowLoad<D, true> lk(lane, p.k.ss);
+  const RowLoad<D, false> lv(lane, p.v.ss);
   const uint32_t lds0 = lds_addr(smem);
-  const RowBase<D> rb(l32, hh);
-  const TrBase<D> tb(lane);
   const int nst = (u.kend - u.kbeg + C::KEYS - 1) / C::KEYS;
   auto issue = [&](int i) {
     const uint32_t dst = lds0 + (i & 1) * 2 * C::TILE;
-    tile_load_async<D, C::KEYS, NW>(u.kg, p.k.ss, u.kbeg + C::KEYS * i, u.kend, dst, wave, lk);
-    tile_load_async<D, C::KEYS, NW>(u.vg, p.v.ss, u.kbeg + C::KEYS * i, u.kend, dst + C::TILE, wave, lv);
+    row_tile_load<D, C::BLOCKS, NW, true>(u.kg, p.k.ss, u.kbeg + C::KEYS * i, u.kend, dst, wave, lane, lk);
+    row_tile_load<D, C::BLOCKS, NW, false>(u.vg, p.v.ss, u.kbeg + C::KEYS * i, u.kend, dst + C::TILE, wave, lane, lv);
   };
   if (nst > 0) issue(0);
-  const float n = *p.n_ptr;
-  const float c = p.scale * *p.b_ptr;
-  RowGroup<T, D> st[1];
+  const float n = u.n, c = u.c;
+  RowGroup<T, D> st;
   const int row = 32 * qw + l32;
-  st[0].init(p, u, row, hh);
+  st.init(p, u, row, hh);
   const bool reaches = nst > 0 && u.kend > u.base;
   if (reaches) pack_mask(p, u, words, tid, NW * 64);
+  if (tid == 0) *bad = 0;
   const uint32_t* mrow =
       words + ((u.row0 + min(row, u.nrows - 1)) / u.G - u.row0 / u.G) * mask_stride(p.T);
   const bool works = 32 * qw < u.nrows;
-  for (int i = 0; i < nst; ++i) {
+  const RowTileK<D> rk(l32, hh);
+  const RowTileV<D> rv(lane);
+  // stages of keys that every row sees, then the rest in a loop of its own (what
+  // only that needs stays out of the first one's registers)
+  const int open = min(u.base, u.kend) - u.kbeg;
+  const int plain = open > 0 ? open / C::KEYS : 0;
+  auto arrive = [&](int i) {
     wait_vm<0>();     // this wave's share of stage i has landed
     __syncthreads();  // and everyone's; everyone is done with the other buffer
     if (i + 1 < nst) issue(i + 1);
+  };
+  int i = 0;
+  for (; i < plain; ++i) {
+    arrive(i);
     if (!works) continue;
-    const uint32_t buf = lds0 + (i & 1) * 2 * C::TILE + kw * BlockLayout<D>::BLOCK;
-    const RowBase<D> kr = at_tile(rb, buf);
-    const TrBase<D> vt = at_tile(tb, buf + C::TILE);
 #pragma unroll
+    for (int t = 0; t < C::U; ++t) {
+      const uint32_t kat = lds0 + (i & 1) * 2 * C::TILE + (kw + KW * t) * RowTile<D>::BLOCK;
+      tree_tile<T, D, NPOS, false>(rk, rv, kat, kat + C::TILE, st, 0, c, n);
+    }
+  }
+#pragma unroll 1
+  for (; i < nst; ++i) {
+    arrive(i);
+    if (!works) continue;
+#pragma unroll 1
     for (int t = 0; t < C::U; ++t) {
       const int key0 = u.kbeg + C::KEYS * i + 32 * (kw + KW * t);
       if (key0 >= u.kend) break;
-      uint32_t win[1] = {0};
+      const uint32_t kat = lds0 + (i & 1) * 2 * C::TILE + (kw + KW * t) * RowTile<D>::BLOCK, vat = kat + C::TILE;
+      uint32_t win = 0xffffffffu;
       if (u.masked(key0)) {
-        win[0] = mask_window(mrow, key0 - u.base) >> (4 * hh);
-        tree_tile<T, D, NPOS, true, 1>(kr, vt, KW * t, st, win, c, n);
-      } else {
-        tree_tile<T, D, NPOS, false, 1>(kr, vt, KW * t, st, win, c, n);
+        win = mask_window(mrow, key0 - u.base);
+        clear_not_finite<T, D>(vat, lane, bad);
       }
+      tree_tile<T, D, NPOS, true>(rk, rv, kat, vat, st, win >> (4 * hh), c, n);
     }
   }
-  float m = st[0].m, l = st[0].l;
-  // the upper half of the key waves hands its (m, l, acc) to the lower, lane by
-  // lane through LDS, until one is left
+  if (reaches) {
+    __syncthreads();  // every wave's tiles have been looked at
+    if (__builtin_expect(*bad != 0, 0))
+      add_not_finite<T, D>(p, u, mrow, u.kbeg + 32 * kw, 32 * KW, hh, st.acc);
+  }
+  float m = st.m, l = st.l;
+  // Each key wave takes a share of the columns: it scales its acc to the common
+  // maximum, hands the others theirs through LDS and adds up its own, the key
+  // waves in order.
+  constexpr int J = C::J, JB = C::JB;
+  f32x4_t mine[JB];
+  const int j0 = kw * JB;  // its float4s of a lane's acc; none where there are more waves than float4s
   if constexpr (KW > 1) {
     f32x4_t* accs = reinterpret_cast<f32x4_t*>(smem);
     float* ml = reinterpret_cast<float*>(words);
+    __syncthreads();  // the stages and masks have been read
+    ml[(2 * wave) * 64 + lane] = m;
+    ml[(2 * wave + 1) * 64 + lane] = l;
+    __syncthreads();
+    float M = -INFINITY;
 #pragma unroll
-    for (int half = KW / 2; half >= 1; half /= 2) {
-      __syncthreads();  // the stages, or the last exchange, have been read
-      const int slot = qw * half + (kw - half);
-      if (works && kw >= half && kw < 2 * half) {
-        ml[(2 * slot) * 64 + lane] = m;
-        ml[(2 * slot + 1) * 64 + lane] = l;
+    for (int w = 0; w < KW; ++w) M = fmaxf(M, ml[(2 * (qw * KW + w)) * 64 + lane]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    l = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4 * ND32; ++j) {
-          f32x4_t x;
+    for (int w = 0; w < KW; ++w)
+      l += ml[(2 * (qw * KW + w) + 1) * 64 + lane] * fast_exp2(ml[(2 * (qw * KW + w)) * 64 + lane] - ref);
+    const float f = fast_exp2(m - ref);
+    m = M;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = st[0].acc[j / 4][4 * (j % 4) + e];
-          accs[(slot * 4 * ND32 + j) * 64 + lane] = x;
-        }
-      }
-      __syncthreads();
-      if (works && kw < half) {
-        const int from = qw * half + kw;
-        const float m2 = ml[(2 * from) * 64 + lane], l2 = ml[(2 * from + 1) * 64 + lane];
-        const float M = fmaxf(m, m2), ref = M == -INFINITY ? 0.f : M;
-        const float f1 = fast_exp2(m - ref), f2 = fast_exp2(m2 - ref);
-        m = M;
-        l = l * f1 + l2 * f2;
+    for (int j = 0; j < J; ++j) {
+      const int owner = j / JB;
+      f32x4_t x;
 #pragma unroll
-        for (int j = 0; j < 4 * ND32; ++j) {
-          const f32x4_t x = accs[(from * 4 * ND32 + j) * 64 + lane];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) st[0].acc[j / 4][4 * (j % 4) + e] = st[0].acc[j / 4][4 * (j % 4) + e] * f1 + x[e] * f2;
-        }
-      }
+      for (int e = 0; e < 4; ++e) x[e] = st.acc[j / 4][4 * (j % 4) + e] * f;
+      if (kw != owner)
+        accs[((qw * J + j) * (KW - 1) + kw - (kw > owner ? 1 : 0)) * 64 + lane] = x;
+      else
+        mine[j % JB] = x;
     }
-    if (kw > 0) return;
+    __syncthreads();
+    if (j0 >= J) return;
+#pragma unroll
+    for (int j = 0; j < JB; ++j) {
+      f32x4_t sum = f32x4_t{};
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        if (w == kw)
+          sum += mine[j];
+        else
+          sum += accs[((qw * J + j0 + j) * (KW - 1) + w - (w > kw ? 1 : 0)) * 64 + lane];
+      }
+      mine[j] = sum;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < JB; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[j][e] = st.acc[j / 4][4 * (j % 4) + e];
+    }
   }
   l = pair_sum(l);
   if (row >= u.nrows) return;
@@ -517,31 +447,20 @@ __device__ __forceinline__ void tree_wide_body(const TreeParams& p, char* smem, 
   if (p.splits == 1) {
     const float l_safe = l == 0.f ? 1.f : l;
     const float inv = 1.f / l_safe;
-    T* dst = static_cast<T*>(const_cast<void*>(p.o.ptr)) + o.off;
+    T* dst = static_cast<T*>(const_cast<void*>(p.o.ptr)) + o.off + 8 * j0 + 4 * hh;
 #pragma unroll
-    for (int db = 0; db < ND32; ++db) {
+    for (int j = 0; j < JB; ++j) {
+      v4 x;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        v4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = static_cast<T>(st[0].acc[db][4 * g + e] * inv);
-        *reinterpret_cast<v4*>(dst + 32 * db + 8 * g + 4 * hh) = x;
-      }
+      for (int e = 0; e < 4; ++e) x[e] = static_cast<T>(mine[j][e] * inv);
+      *reinterpret_cast<v4*>(dst + 8 * j) = x;
     }
-    if (hh == 0 && p.m != nullptr) p.m[o.mrow] = m + log2f(l_safe);
+    if (kw == 0 && hh == 0 && p.m != nullptr) p.m[o.mrow] = m + log2f(l_safe);
   } else {
-    float* dst = p.ws_acc + o.rec * D;
+    float* dst = p.ws_acc + o.rec * D + 8 * j0 + 4 * hh;
 #pragma unroll
-    for (int db = 0; db < ND32; ++db) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4_t x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = st[0].acc[db][4 * g + e];
-        *reinterpret_cast<f32x4_t*>(dst + 32 * db + 8 * g + 4 * hh) = x;
-      }
-    }
-    if (hh == 0) {
+    for (int j = 0; j < JB; ++j) *reinterpret_cast<f32x4_t*>(dst + 8 * j) = mine[j];
+    if (kw == 0 && hh == 0) {
       p.ws_ml[2 * o.rec] = m;
       p.ws_ml[2 * o.rec + 1] = l;
     }
@@ -550,32 +469,19 @@ __device__ __forceinline__ void tree_wide_body(const TreeParams& p, char* smem, 
 
 }  // namespace
 
-template <typename T, int D, int NQ>
-__global__ __launch_bounds__(DecodeCfg<D>::NW * 64) void tree_stream_kernel(TreeParams p, int nunits) {
-  __shared__ __attribute__((aligned(1024))) char smem[DecodeCfg<D>::SMEM];
-  __shared__ uint32_t words[32 * NQ * kMaskWords];
-  const int block = folded_block();
-  if (block >= nunits) return;
-  const TreeUnit u(p, block, 32 * NQ, 1);
-  if (p.splits > 1 && u.kend <= u.kbeg) return;  // a shorter sequence: nothing to merge
-  if (*p.n_ptr >= 0.f)
-    tree_stream_body<T, D, true, NQ>(p, smem, words, u);
-  else
-    tree_stream_body<T, D, false, NQ>(p, smem, words, u);
-}
-
 template <typename T, int D, int QW, int KW>
-__global__ __launch_bounds__(QW* KW * 64) void tree_wide_kernel(TreeParams p, int nunits, int nqb) {
-  __shared__ __attribute__((aligned(1024))) char smem[WideCfg<D, QW, KW>::SMEM];
-  __shared__ uint32_t words[32 * QW * kMaskWords];
+__global__ __launch_bounds__(QW* KW * 64) void tree_kernel(TreeParams p, int nunits, int nqb) {
+  __shared__ __attribute__((aligned(1024))) char smem[TreeCfg<D, QW, KW>::SMEM];
+  __shared__ uint32_t words[TreeCfg<D, QW, KW>::WORDS];  // packed masks; later the key waves' m and l
+  __shared__ int bad;  // the tree's rows of V held an infinity or NaN
   const int block = folded_block();
   if (block >= nunits) return;
   const TreeUnit u(p, block, 32 * QW, nqb);
   if (p.splits > 1 && u.kend <= u.kbeg) return;  // a shorter sequence: nothing to merge
-  if (*p.n_ptr >= 0.f)
-    tree_wide_body<T, D, true, QW, KW>(p, smem, words, u);
+  if (u.n >= 0.f)
+    tree_body<T, D, true, QW, KW>(p, smem, words, &bad, u);
   else
-    tree_wide_body<T, D, false, QW, KW>(p, smem, words, u);
+    tree_body<T, D, false, QW, KW>(p, smem, words, &bad, u);
 }
 
 // The splits' partials of a row in split order: out = sum_s acc_s 2^(m_s - M) /
@@ -597,15 +503,20 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p, int nrows
   const int ns = static_cast<int>((L + p.split_keys - 1) / p.split_keys);  // the sequence's own splits
   const int64_t rec0 = static_cast<int64_t>(row) * p.splits;
   const float* ml = p.ws_ml + 2 * rec0;
+  // the row's lanes of a wave take a split each for the maximum and the sum
+  constexpr int LANES = TPR * SW < 64 ? TPR * SW : 64;
+  const int at = tid % LANES;
   float M = -INFINITY;
-#pragma unroll 4
-  for (int s = 0; s < ns; ++s) M = fmaxf(M, ml[2 * s]);
+  for (int s = at; s < ns; s += LANES) M = fmaxf(M, ml[2 * s]);
+#pragma unroll
+  for (int off = LANES / 2; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
   const float ref = M == -INFINITY ? 0.f : M;
   float Ls = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < ns; ++s) Ls += ml[2 * s + 1] * fast_exp2(ml[2 * s] - ref);
+  for (int s = at; s < ns; s += LANES) Ls += ml[2 * s + 1] * fast_exp2(ml[2 * s] - ref);
+#pragma unroll
+  for (int off = LANES / 2; off > 0; off >>= 1) Ls += __shfl_xor(Ls, off, 64);
   f32x4_t O = f32x4_t{};
-#pragma unroll 4
+#pragma unroll 8
   for (int s = sw; s < ns; s += SW)
     O += *reinterpret_cast<const f32x4_t*>(p.ws_acc + (rec0 + s) * D + col) * fast_exp2(ml[2 * s] - ref);
   if constexpr (SW > 1) {
@@ -639,16 +550,18 @@ hipError_t launch_tree_t(const TreeParams& p, hipStream_t s) {
   const int per = tree_rows_per_block(rows);
   const int nqb = static_cast<int>((rows + per - 1) / per);
   const int units = static_cast<int>(tree_units(p.B, p.Hq, p.Hkv, p.T) * p.splits);
-  constexpr int ST = DecodeCfg<D>::NW * 64;
-  constexpr int WT = D == 128 ? 512 : 1024, KW = D == 128 ? 1 : 2;  // threads; key waves of 8 row groups
+  const auto go = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, folded_grid(units, threads), dim3(threads), 0, s, p, units, nqb);
+  };
+  constexpr int W = D == 128 ? 8 : 16;  // waves of a workgroup: 128 KB of LDS, 128 or 256 registers
   if (per == 32)
-    hipLaunchKernelGGL((tree_stream_kernel<T, D, 1>), folded_grid(units, ST), dim3(ST), 0, s, p, units);
+    go(tree_kernel<T, D, 1, W / 2>, W / 2 * 64);
   else if (per == 64)
-    hipLaunchKernelGGL((tree_stream_kernel<T, D, 2>), folded_grid(units, ST), dim3(ST), 0, s, p, units);
+    go(tree_kernel<T, D, 2, W / 2>, W * 64);
   else if (per == 128)
-    hipLaunchKernelGGL((tree_wide_kernel<T, D, 4, 2 * KW>), folded_grid(units, WT), dim3(WT), 0, s, p, units, nqb);
+    go(tree_kernel<T, D, 4, W / 4>, W * 64);
   else
-    hipLaunchKernelGGL((tree_wide_kernel<T, D, 8, KW>), folded_grid(units, WT), dim3(WT), 0, s, p, units, nqb);
+    go(tree_kernel<T, D, 8, W / 8>, W * 64);
   if (p.splits > 8)
     launch_merge<T, D, 4>(p, s);
   else if (p.splits > 1)
