@@ -72,12 +72,16 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* waves, int 
 }  // namespace
 
 // A wave takes 64 E consecutive rows, four consecutive ones a lane at a time, a
-// workgroup 1024 E: a cache of up to that many rows is read once and its keys
-// stay in registers for every pass, a longer one is read by each.  Rows that
-// stay in any case rank above every weight and rows past the length below or
-// with the lowest, where the lower row wins.
-template <int E>
+// workgroup a stretch of 1024 E.  The first stretch's keys stay in registers for
+// every pass, with kFar the second's in LDS; a cache longer than that (65536 rows
+// at E = 32) is read by every pass from there on.  Rows that stay in any case rank
+// above every weight, rows past the length with the lowest, where the lower row
+// wins.
+template <int E, bool kFar = false>
 __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams p, int nblocks) {
+  constexpr int STRETCH = kSelect * E;
+  constexpr uint32_t kMust = 0xffffffffu;
+  __shared__ __attribute__((aligned(16))) uint32_t far[kFar ? STRETCH : 4];
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t waves[kSelect / 64];
   __shared__ uint32_t found[2];  // digit, rows above it
@@ -95,160 +99,214 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams p, in
     for (int i = tid; i < p.keep; i += kSelect) kept[i] = i < L ? i : -1;
     return;
   }
-  constexpr int STRETCH = kSelect * E;
   const int mine = wave * 64 * E + 4 * lane;  // the lane's first row of a stretch; then every 256th
   const int lo = p.sinks, hi = L - p.recent;  // rows [lo, hi) are chosen from
+  const int stretches = (L - 1) / STRETCH + 1;
+  auto load = [&](int i, uint32_t* k) {  // the keys of rows i .. i + 3
+    f32x4_u x = {0.f, 0.f, 0.f, 0.f};
+    if (i + 3 < L) {
+      x = *reinterpret_cast<const f32x4_u*>(w + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < L) x[e] = w[i + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) k[e] = i + e >= L ? 0u : (i + e < lo || i + e >= hi) ? kMust : order_bits(x[e]);
+  };
   uint32_t key[E];
-  auto load = [&](int r0) {
 #pragma unroll
+  for (int j = 0; j < E / 4; ++j) load(mine + 256 * j, key + 4 * j);
+  u32x4* far4 = reinterpret_cast<u32x4*>(far);
+  if (kFar && stretches > 1) {
+#pragma unroll 4
     for (int j = 0; j < E / 4; ++j) {
-      const int i = r0 + mine + 256 * j;
-      f32x4_u x = {0.f, 0.f, 0.f, 0.f};
-      if (i + 3 < L) {
-        x = *reinterpret_cast<const f32x4_u*>(w + i);
-      } else {
+      uint32_t k[4];
+      load(STRETCH + mine + 256 * j, k);
+      far4[kSelect * j + tid] = u32x4{k[0], k[1], k[2], k[3]};  // read by this thread only
+    }
+  }
+  // f(first of four rows, their keys) for the lane's rows of stretch s, in order;
+  // not for 256 rows past the length (a histogram's lowest bin would take them
+  // one by one)
+  const int wave0 = __builtin_amdgcn_readfirstlane(wave * 64 * E);
+  auto each = [&](int s, auto&& f) {
+    if (s == 0) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i + e < L) x[e] = w[i + e];
-      }
+      for (int j = 0; j < E / 4; ++j)
+        if (wave0 + 256 * j < L) f(mine + 256 * j, key + 4 * j);
+    } else {
+      const int r0 = s * STRETCH + mine;  // below 2^30 + 2^15
+#pragma unroll 2
+      for (int j = 0; j < E / 4; ++j) {
+        if (s * STRETCH + wave0 + 256 * j >= L) break;
+        uint32_t k[4];
+        if (kFar && s == 1) {
+          const u32x4 v = far4[kSelect * j + tid];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t k = order_bits(x[e]);
-        key[4 * j + e] = i + e >= L ? 0u : (i + e < lo || i + e >= hi) ? 0xffffffffu : k;
+          for (int e = 0; e < 4; ++e) k[e] = v[e];
+        } else {
+          load(r0 + 256 * j, k);
+        }
+        f(r0 + 256 * j, k);
       }
     }
   };
-  const bool once = L <= STRETCH;
-  if (once) load(0);
-  for (int i = p.keep + tid; i < p.cap; i += kSelect) w_out[i] = 0.f;
-  uint32_t need = p.keep;  // rows that stay, of those that share the prefix
+  uint32_t need = p.keep - p.sinks - p.recent;  // rows that stay, of those that share the prefix
   uint32_t prefix = 0;
-  constexpr int kShift[3] = {20, 10, 0}, kWidth[3] = {12, 10, 10};
+  if (need == 0) {
+    prefix = kMust;
+    need = p.keep;
+  } else {
+    constexpr int kShift[3] = {20, 10, 0}, kWidth[3] = {12, 10, 10};
 #pragma unroll
-  for (int pass = 0; pass < 3; ++pass) {
-    const int bins = 1 << kWidth[pass];
-    for (int i = tid; i < bins; i += kSelect) hist[i] = 0;
-    __syncthreads();
-    for (int r0 = 0; r0 < L; r0 += STRETCH) {
-      if (!once) load(r0);
+    for (int pass = 0; pass < 3; ++pass) {
+      const int bins = 1 << kWidth[pass];
+      for (int i = tid; i < bins; i += kSelect) hist[i] = 0;
+      __syncthreads();
+      for (int s = 0; s < stretches; ++s)
+        each(s, [&](int, const uint32_t* k) {
 #pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (pass == 0 || (key[j] >> (kShift[pass] + kWidth[pass])) == prefix)
-          atomicAdd(&hist[(key[j] >> kShift[pass]) & (bins - 1)], 1u);
+          for (int e = 0; e < 4; ++e)
+            if (k[e] != kMust && (pass == 0 || (k[e] >> (kShift[pass] + kWidth[pass])) == prefix))
+              atomicAdd(&hist[(k[e] >> kShift[pass]) & (bins - 1)], 1u);
+        });
+      __syncthreads();
+      // bins from the top: thread i takes `per` bins downwards from the i-th group
+      const int per = bins / kSelect;
+      uint32_t sum = 0;
+      for (int x = 0; x < per; ++x) sum += hist[bins - 1 - per * tid - x];
+      uint32_t total;
+      const uint32_t upto = block_scan(sum, waves, tid, total);
+      uint32_t above = upto - sum;
+      if (above < need && upto >= need) {
+        int bin = bins - 1 - per * tid;
+        while (above + hist[bin] < need) above += hist[bin--];
+        found[0] = bin;
+        found[1] = above;
+      }
+      __syncthreads();
+      prefix = (prefix << kWidth[pass]) | found[0];
+      need -= found[1];
     }
-    __syncthreads();
-    // bins from the top: thread i takes `per` bins downwards from the i-th group
-    const int per = bins / kSelect;
-    uint32_t sum = 0;
-    for (int x = 0; x < per; ++x) sum += hist[bins - 1 - per * tid - x];
-    uint32_t total;
-    const uint32_t upto = block_scan(sum, waves, tid, total);
-    uint32_t above = upto - sum;
-    if (above < need && upto >= need) {
-      int bin = bins - 1 - per * tid;
-      while (above + hist[bin] < need) above += hist[bin--];
-      found[0] = bin;
-      found[1] = above;
-    }
-    __syncthreads();
-    prefix = (prefix << kWidth[pass]) | found[0];
-    need -= found[1];
   }
   const uint32_t ties = need;  // rows at the threshold that stay, the lowest first
   uint32_t above0 = 0, at0 = 0;  // rows before this stretch above the threshold; at it
-  for (int r0 = 0; r0 < L; r0 += STRETCH) {
-    if (!once) load(r0);
+  for (int s = 0; s < stretches; ++s) {
     // the wave's counts: above in the low half, at the threshold in the high
-    uint32_t up = 0, eq = 0;
+    uint32_t both = 0;
+    each(s, [&](int, const uint32_t* k) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      up += key[j] > prefix;
-      eq += key[j] == prefix;
-    }
+      for (int e = 0; e < 4; ++e) both += (k[e] > prefix) + ((k[e] == prefix) << 16);
+    });
     // a wave's 64 E rows are at most 2^11, a workgroup's at most 2^15: no carry
-    uint32_t total, before_waves = 0;
-    {
-      const uint32_t sum = wave_scan(up | (eq << 16));
-      __syncthreads();
-      if (lane == 63) waves[wave] = sum;
-      __syncthreads();
-      total = 0;
+    uint32_t total = 0, before_waves = 0;
+    const uint32_t sum = wave_scan(both);
+    __syncthreads();
+    if (lane == 63) waves[wave] = sum;
+    __syncthreads();
 #pragma unroll
-      for (int x = 0; x < kSelect / 64; ++x) {
-        before_waves += x < wave ? waves[x] : 0;
-        total += waves[x];
-      }
+    for (int x = 0; x < kSelect / 64; ++x) {
+      before_waves += x < wave ? waves[x] : 0;
+      total += waves[x];
     }
-#pragma unroll
-    for (int j = 0; j < E / 4; ++j) {
+    each(s, [&](int i, const uint32_t* k) {
       uint32_t count = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) count += (key[4 * j + e] > prefix) + ((key[4 * j + e] == prefix) << 16);
+      for (int e = 0; e < 4; ++e) count += (k[e] > prefix) + ((k[e] == prefix) << 16);
       const uint32_t upto = wave_scan(count);
       uint32_t before = before_waves + upto - count;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bool over = key[4 * j + e] > prefix, even = key[4 * j + e] == prefix;
+        const bool over = k[e] > prefix, even = k[e] == prefix;
         const uint32_t at = at0 + (before >> 16), place = above0 + (before & 0xffffu) + (at < ties ? at : ties);
-        if (over || (even && at < ties)) {
-          const int i = r0 + mine + 256 * j + e;
-          kept[place] = i;
-          w_out[place] = w[i];
-        }
+        if (over || (even && at < ties)) kept[place] = i + e;
         before += over + (even << 16);
       }
       before_waves += __builtin_amdgcn_readlane(upto, 63);
-    }
+    });
     above0 += total & 0xffffu;
     at0 += total >> 16;
   }
+  // behind the kept rows' weights, which evict_move_kernel gathers
+  const int n4 = (p.cap - p.keep) / 4;
+  for (int i = tid; i < n4; i += kSelect)
+    *reinterpret_cast<f32x4_u*>(w_out + p.keep + 4 * static_cast<int64_t>(i)) = f32x4_u{0.f, 0.f, 0.f, 0.f};
+  if (tid < (p.cap - p.keep) % 4) w_out[p.keep + 4 * static_cast<int64_t>(n4) + tid] = 0.f;
 }
 
-// One workgroup per (tensor, sequence, kv-head, slice of SP 16-byte pieces of a
-// row), the slices of a head on one XCD.  The next chunk's rows are on their way
-// while this one's are written.
-template <int SP>
+// One workgroup per (sequence, kv-head) that gathers the kept rows' weights, then
+// one per (tensor, sequence, kv-head, slice of SP 16-byte pieces of a row), the
+// slices of a head on one XCD.  The next chunk's rows are on their way while
+// this one's are written.
+template <int SP, int U>
 __global__ __launch_bounds__(1024) void evict_move_kernel(EvictParams p, int slices, int nblocks) {
-  constexpr int U = 4, ROWS = 1024 / SP;  // rows of one step, U steps a chunk
-  const int block = folded_block();
+  constexpr int ROWS = 1024 / SP, CHUNK = U * ROWS;  // rows of one step, U steps a chunk
+  const int heads = p.B * p.Hkv, tid = threadIdx.x;
+  int block = folded_block();
   if (block >= nblocks) return;
-  const int units = nblocks / slices;
-  const int slice = block / units;
-  int u = block - slice * units;
-  const Tensor4& t = (u & 1) ? p.v : p.k;
-  u >>= 1;
+  const bool weighs = block < heads;
+  block -= heads;
+  const int units = 2 * heads, slice = weighs ? 0 : block / units;
+  int u = weighs ? block + heads : block - slice * units;
+  const bool is_v = u & 1;
+  if (!weighs) u >>= 1;
   const int h = u % p.Hkv, b = u / p.Hkv;
-  const int L = clamped_len(p.seqlens, b, p.cap);
-  if (L <= p.keep) return;
+  if (clamped_len(p.seqlens, b, p.cap) <= p.keep) return;
   const int* kept = p.kept + static_cast<int64_t>(u) * p.keep;
-  const int tid = threadIdx.x, piece = slice * SP + tid % SP, row = tid / SP;
+  if (weighs) {
+    const float* w = p.w + b * p.w_sb + h * p.w_sh;
+    float* w_out = p.w_out + static_cast<int64_t>(u) * p.cap;
+    for (int64_t r0 = tid; r0 < p.keep; r0 += 8 * 1024) {
+      int src[8];
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) src[j] = kept[r0 + 1024 * j < p.keep ? r0 + 1024 * j : p.keep - 1];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = w[src[j]];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (r0 + 1024 * j < p.keep) w_out[r0 + 1024 * j] = x[j];
+    }
+    return;
+  }
+  const Tensor4& t = is_v ? p.v : p.k;
+  const int piece = slice * SP + tid % SP, row = tid / SP;
   char* base = static_cast<char*>(const_cast<void*>(t.ptr)) + (b * t.sb + h * t.sh) * 2 + piece * 16;
   const int64_t step = t.ss * 2;
+  // kept[r] - r never falls: a chunk whose last row stays in place stays whole
+  int r0 = 0;
+  while (r0 < p.keep) {
+    const int last = (p.keep - r0 < CHUNK ? p.keep : r0 + CHUNK) - 1;
+    if (load_table_entry(kept, last) != last) break;
+    r0 = last + 1;
+  }
   u32x4 v[U], next[U];
   int src[U];
-  auto index = [&](int r0) {
+  auto index = [&](int at) {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int r = r0 + j * ROWS + row;
+      const int r = at + j * ROWS + row;
       src[j] = r < p.keep ? kept[r] : r;
     }
   };
-  auto fetch = [&](u32x4 (&to)[U], int r0) {
+  auto fetch = [&](u32x4 (&to)[U], int at) {
 #pragma unroll
     for (int j = 0; j < U; ++j)
-      if (src[j] != r0 + j * ROWS + row) to[j] = *reinterpret_cast<const u32x4*>(base + src[j] * step);
+      if (src[j] != at + j * ROWS + row) to[j] = *reinterpret_cast<const u32x4*>(base + src[j] * step);
   };
-  index(0);
-  fetch(v, 0);
-  for (int r0 = 0; r0 < p.keep; r0 += U * ROWS) {
+  if (r0 >= p.keep) return;
+  index(r0);
+  fetch(v, r0);
+  for (; r0 < p.keep; r0 += CHUNK) {  // below 2^30 + CHUNK
     bool moves[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) moves[j] = src[j] != r0 + j * ROWS + row;
-    const bool more = r0 + U * ROWS < p.keep;
-    if (more) index(r0 + U * ROWS);
+    const bool more = p.keep - r0 > CHUNK;
+    if (more) index(r0 + CHUNK);
     __builtin_amdgcn_s_waitcnt(0);  // the chunk's rows are in registers ...
     __syncthreads();                // ... everywhere
-    if (more) fetch(next, r0 + U * ROWS);
+    if (more) fetch(next, r0 + CHUNK);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int r = r0 + j * ROWS + row;
@@ -308,17 +366,21 @@ hipError_t launch_evict(const EvictParams& p, hipStream_t s) {
     hipLaunchKernelGGL(evict_select_kernel<4>, grid, dim3(kSelect), 0, s, p, heads);
   else if (p.cap <= 16 * kSelect)
     hipLaunchKernelGGL(evict_select_kernel<16>, grid, dim3(kSelect), 0, s, p, heads);
-  else
+  else if (p.cap <= 32 * kSelect)
     hipLaunchKernelGGL(evict_select_kernel<32>, grid, dim3(kSelect), 0, s, p, heads);
+  else
+    hipLaunchKernelGGL((evict_select_kernel<32, true>), grid, dim3(kSelect), 0, s, p, heads);
+  // 64-byte slices move at the rate of a copy where they fill the GPU (512 and 1152
+  // workgroups; slices of 32 bytes take 1.7 times as long); up to 128 workgroups
+  // half the slice on twice as many is 20 to 25 % shorter
   const auto move = [&](auto kernel, int sp) {
-    const int slices = p.D / 8 / sp;
-    const int blocks = heads * 2 * slices;
+    const int slices = p.D / 8 / sp, blocks = heads * (1 + 2 * slices);
     hipLaunchKernelGGL(kernel, folded_grid(blocks, 1024), dim3(1024), 0, s, p, slices, blocks);
   };
-  if (heads * 2 * (p.D / 32) < 256)
-    move(evict_move_kernel<2>, 2);
+  if (heads * 2 * (p.D / 32) <= 128)
+    move(evict_move_kernel<2, 8>, 2);
   else
-    move(evict_move_kernel<4>, 4);
+    move(evict_move_kernel<4, 4>, 4);
   return hipGetLastError();
 }
 

@@ -99,13 +99,23 @@ __device__ __forceinline__ void pack_mask(const TreeParams& p, const TreeUnit& u
   const int lane = tid & 63, W = mask_stride(p.T), chunks = (p.T + 63) / 64;
   const int n0 = u.row0 / u.G, nn = (u.row0 + u.nrows - 1) / u.G - n0 + 1;
   const uint8_t* mask = p.mask + u.b * p.mask_sb + static_cast<int64_t>(n0) * p.T;
-  for (int i = tid >> 6; i < nn * chunks; i += nthreads >> 6) {
-    const int n = i / chunks, c = i - n * chunks, col = 64 * c + lane;
-    const uint64_t bits = __ballot(col < p.T && mask[n * p.T + col] != 0);
-    if (lane == 0) {
-      words[n * W + 2 * c] = static_cast<uint32_t>(bits);
-      words[n * W + 2 * c + 1] = static_cast<uint32_t>(bits >> 32);
-      if (c == chunks - 1) words[n * W + 2 * chunks] = 0;
+  const int waves = nthreads >> 6;
+  for (int i0 = tid >> 6; i0 < nn * chunks; i0 += 4 * waves) {
+    uint8_t byte[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {  // four loads on their way at a time
+      const int i = i0 + x * waves, n = i / chunks, col = 64 * (i - n * chunks) + lane;
+      byte[x] = i < nn * chunks && col < p.T ? mask[n * p.T + col] : 0;
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = i0 + x * waves, n = i / chunks, c = i - n * chunks;
+      const uint64_t bits = __ballot(byte[x] != 0);
+      if (lane == 0 && i < nn * chunks) {
+        words[n * W + 2 * c] = static_cast<uint32_t>(bits);
+        words[n * W + 2 * c + 1] = static_cast<uint32_t>(bits >> 32);
+        if (c == chunks - 1) words[n * W + 2 * chunks] = 0;
+      }
     }
   }
 }
@@ -178,19 +188,25 @@ __device__ __forceinline__ void clear_not_finite(uint32_t vat, int lane, int* ba
   }
 }
 
-// One tile of 32 keys (blocks at kat and vat) for the wave's 32 rows: scores,
-// transform, softmax update and the product with V.  MASKED: win holds the keys
-// that the lane's row sees, shifted by 4 hh.
-template <typename T, int D, bool NPOS, bool MASKED>
-__device__ __forceinline__ void tree_tile(const RowTileK<D>& rk, const RowTileV<D>& rv, uint32_t kat, uint32_t vat,
-                                          RowGroup<T, D>& st, uint32_t win, float c, float n) {
-  typedef typename Vec8<T>::type v8;
-  typedef T v4 __attribute__((ext_vector_type(4)));
-  constexpr int ND16 = D / 16, ND32 = D / 32;
-  constexpr uint32_t kOut = NPOS ? 0xff800000u : 0x7f800000u;  // the score of the lowest t: -inf or +inf
+// q.k of the wave's 32 rows and a block of 32 keys at kat.
+template <typename T, int D>
+__device__ __forceinline__ f32x16 tree_scores(const RowTileK<D>& rk, uint32_t kat, const RowGroup<T, D>& st) {
   f32x16 s = f32x16{};
 #pragma unroll
-  for (int ds = 0; ds < ND16; ++ds) s = mfma32(rk.template read<v8>(kat, ds), st.q[ds], s);
+  for (int ds = 0; ds < D / 16; ++ds) s = mfma32(rk.template read<typename Vec8<T>::type>(kat, ds), st.q[ds], s);
+  return s;
+}
+
+// One tile of 32 keys for the wave's 32 rows: transform of its scores, softmax
+// update and the product with its block of V at vat.  MASKED: win holds the keys
+// that the lane's row sees, shifted by 4 hh.
+template <typename T, int D, bool NPOS, bool MASKED>
+__device__ __forceinline__ void tree_tile(f32x16 s, const RowTileV<D>& rv, uint32_t vat, RowGroup<T, D>& st,
+                                          uint32_t win, float c, float n) {
+  typedef typename Vec8<T>::type v8;
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  constexpr int ND32 = D / 32;
+  constexpr uint32_t kOut = NPOS ? 0xff800000u : 0x7f800000u;  // the score of the lowest t: -inf or +inf
   v8 pb[2];
   bool done = false;
   if constexpr (!MASKED) {
@@ -300,7 +316,9 @@ struct RowOut {
 template <int D, int QW, int KW>
 struct TreeCfg {
   static constexpr int NW = QW * KW;
-  static constexpr int U = KW == 1 ? 2 : 1;  // tiles of a wave and stage
+  // tiles of a wave and stage: two where that leaves the stage at 64 KB (a longer
+  // first stage costs a short range of keys more than its barriers)
+  static constexpr int U = 2 * KW * 2 * RowTile<D>::BLOCK <= 40 * 1024 ? 2 : 1;
   static constexpr int BLOCKS = KW * U;
   static constexpr int KEYS = 32 * BLOCKS;
   static constexpr int TILE = BLOCKS * RowTile<D>::BLOCK;
@@ -357,10 +375,20 @@ __device__ __forceinline__ void tree_body(const TreeParams& p, char* smem, uint3
   for (; i < plain; ++i) {
     arrive(i);
     if (!works) continue;
+    const uint32_t kat = lds0 + (i & 1) * 2 * C::TILE + kw * RowTile<D>::BLOCK;
+    const auto scores = [&](int t) { return tree_scores(rk, kat + KW * t * RowTile<D>::BLOCK, st); };
+    const auto rest = [&](const f32x16& s, int t) {
+      tree_tile<T, D, NPOS, false>(s, rv, kat + C::TILE + KW * t * RowTile<D>::BLOCK, st, 0, c, n);
+    };
+    if constexpr (C::U == 2 && D != 64) {
+      // the second tile's scores are on the matrix cores while the first's go
+      // through the transform (at D = 64 that would not fit 128 registers)
+      const f32x16 s0 = scores(0), s1 = scores(1);
+      rest(s0, 0);
+      rest(s1, 1);
+    } else {
 #pragma unroll
-    for (int t = 0; t < C::U; ++t) {
-      const uint32_t kat = lds0 + (i & 1) * 2 * C::TILE + (kw + KW * t) * RowTile<D>::BLOCK;
-      tree_tile<T, D, NPOS, false>(rk, rv, kat, kat + C::TILE, st, 0, c, n);
+      for (int t = 0; t < C::U; ++t) rest(scores(t), t);
     }
   }
 #pragma unroll 1
@@ -377,7 +405,7 @@ __device__ __forceinline__ void tree_body(const TreeParams& p, char* smem, uint3
         win = mask_window(mrow, key0 - u.base);
         clear_not_finite<T, D>(vat, lane, bad);
       }
-      tree_tile<T, D, NPOS, true>(rk, rv, kat, vat, st, win >> (4 * hh), c, n);
+      tree_tile<T, D, NPOS, true>(tree_scores(rk, kat, st), rv, vat, st, win >> (4 * hh), c, n);
     }
   }
   if (reaches) {
