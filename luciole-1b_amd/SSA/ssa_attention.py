@@ -22,7 +22,10 @@ Generation: ``SSAKVCache`` + ``SSAAttention.forward_decode`` run one token
 per step against the cached keys and values (the decode kernel), where the
 reference's generation loop re-runs the whole prefix through the forward for
 every token (training/train/train_ssa_triton/generate_triton.py:315-331); the
-result is the same causal attention row.
+result is the same causal attention row.  A drafted tree of tokens is checked
+in one step (``forward_tree``, then ``SSAKVCache.accept`` for the path that was
+right), and a cache that tracks its keys' accumulated attention weights
+(``track_weights``) can be cut to a budget (``SSAKVCache.evict``).
 """
 
 from __future__ import annotations
@@ -33,8 +36,9 @@ from typing import Optional
 import torch
 from torch import nn
 
+from .ssa_cache_ops import ssa_cache_accept, ssa_cache_evict, ssa_key_weights, ssa_tree_attention
 from .ssa_flash_attention import ssa_flash_attention, ssa_flash_attention_varlen
-from .ssa_hip_kernel import ssa_decode_attention
+from .ssa_hip_kernel import ssa_decode_attention, ssa_flash_attn_forward
 
 
 class SSAKVCache:
@@ -45,17 +49,26 @@ class SSAKVCache:
     sequence.  Appends write at each sequence's own length without a host
     synchronisation; positions past ``capacity`` are clamped to its last row,
     so the caller sizes the cache for the longest generation.
+
+    With ``track_weights``, ``weights`` (fp32 ``[B, Hkv, capacity]``) holds the
+    attention that the queries so far paid to every cached key (0 behind the
+    sequence); ``SSAAttention`` keeps it up to date, and ``evict`` cuts the
+    cache by it.
     """
 
     def __init__(self, batch: int, heads_kv: int, capacity: int, head_dim: int, dtype=torch.bfloat16,
-                 device="cuda"):
+                 device="cuda", track_weights: bool = False):
         self.k = torch.zeros(batch, heads_kv, capacity, head_dim, dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
         self.seqlens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.capacity = capacity
+        self.weights = (torch.zeros(batch, heads_kv, capacity, dtype=torch.float32, device=device)
+                        if track_weights else None)
+        self._drafted = None  # (q, m, scale, n, b) of the last drafted tree, for the weights of its accepted path
 
     def append(self, key: torch.Tensor, value: torch.Tensor) -> None:
         """Append ``T`` new tokens per sequence: key / value ``[B, Hkv, T, D]``."""
+        self._drafted = None
         B, _, T, _ = key.shape
         pos = self.seqlens.long().unsqueeze(1) + torch.arange(T, device=key.device).unsqueeze(0)
         pos = pos.clamp_(max=self.capacity - 1)
@@ -64,6 +77,52 @@ class SSAKVCache:
         self.k[bidx, :, pos] = key.transpose(1, 2).to(self.k.dtype)
         self.v[bidx, :, pos] = value.transpose(1, 2).to(self.v.dtype)
         self.seqlens += T
+
+    def add_weights(self, q: torch.Tensor, m: torch.Tensor, softmax_scale, ssa_n, ssa_b) -> None:
+        """Adds the attention that the last queries (``[B, Hq, T, D]`` or ``[B, Hq,
+        D]``, ``m`` their normalisers) paid to the cached keys
+        (``ssa_key_weights``)."""
+        if self.weights is None:
+            raise ValueError("the cache does not track weights (track_weights=True)")
+        ssa_key_weights(q, self.k, m, self.seqlens, self.weights, softmax_scale, ssa_n, ssa_b)
+
+    def evict(self, keep: int, sinks: int = 0, recent: int = 0) -> torch.Tensor:
+        """Cuts every sequence of more than ``keep`` rows to ``keep`` of them, by
+        weight, the first ``sinks`` and last ``recent`` rows in any case
+        (``ssa_cache_evict``); returns the rows that stayed, int32 ``[B, Hkv,
+        keep]``, -1 behind the last."""
+        if self.weights is None:
+            raise ValueError("the cache does not track weights (track_weights=True)")
+        self._drafted = None
+        lens, weights, kept = ssa_cache_evict(self.k, self.v, self.seqlens, self.weights, keep, sinks, recent)
+        self.seqlens.copy_(lens)
+        self.weights.copy_(weights)
+        return kept
+
+    def accept(self, path: torch.Tensor, accepted: torch.Tensor, nodes: int) -> None:
+        """Keeps of the last ``nodes`` rows, a drafted tree's, the first
+        ``accepted[b]`` nodes of ``path[b]``, in that order
+        (``ssa_cache_accept``).  A tracking cache gains the attention that the
+        accepted tokens paid."""
+        drafted, self._drafted = self._drafted, None
+        path = torch.as_tensor(path, device=self.k.device).to(torch.int32)
+        accepted = torch.as_tensor(accepted, device=self.k.device).to(torch.int32)
+        held = self.seqlens >= nodes
+        self.seqlens.copy_(ssa_cache_accept(self.k, self.v, self.seqlens, path, accepted, nodes))
+        if self.weights is None or drafted is None:
+            return
+        q, m, scale, n, b = drafted
+        if q.shape[2] != nodes:
+            raise ValueError(f"the last tree had {q.shape[2]} nodes, not {nodes}")
+        # the path's queries at the end of the sequence, rows that were not accepted before them
+        depth = path.shape[1]
+        count = torch.where(held, accepted.clamp(0, depth), torch.zeros_like(accepted)).long()
+        step = torch.arange(depth, device=path.device)[None, :] - (depth - count)[:, None]
+        node = path.long().clamp(0, nodes - 1).gather(1, step.clamp_min(0))
+        at = node[:, None, :].expand(-1, q.shape[1], -1)
+        rows = q.gather(2, at[..., None].expand(-1, -1, -1, q.shape[3]))
+        norm = m.gather(2, at).masked_fill((step < 0)[:, None, :], -math.inf)
+        ssa_key_weights(rows, self.k, norm, self.seqlens, self.weights, scale, n, b)
 
 
 class SSAAttention(nn.Module):
@@ -148,5 +207,43 @@ class SSAAttention(nn.Module):
             raise ValueError("forward_decode takes one new token per sequence ([1, B, H, D])")
         n, b = self.get_ssa_params()
         cache.append(key.permute(1, 2, 0, 3), value.permute(1, 2, 0, 3))
-        ctx = ssa_decode_attention(query[0], cache.k, cache.v, cache.seqlens, self.softmax_scale, n, b)
+        track = cache.weights is not None
+        ctx = ssa_decode_attention(query[0], cache.k, cache.v, cache.seqlens, self.softmax_scale, n, b,
+                                   return_m=track)
+        if track:
+            ctx, m = ctx
+            cache.add_weights(query[0], m, self.softmax_scale, n, b)
         return ctx.reshape(1, query.shape[1], -1)
+
+    @torch.no_grad()
+    def forward_prompt(self, query, key, value, cache: SSAKVCache, window: Optional[int] = None):
+        """A prompt into an empty cache: query [S, B, Hq, D], key/value [S, B, Hkv, D]
+        -> context [S, B, Hq * D] of the dense causal forward, without
+        gradients; keys and values go to ``cache``, and a tracking cache gains
+        the attention that the last ``window`` tokens (None: all) paid."""
+        n, b = self.get_ssa_params()
+        q, k, v = (t.permute(1, 2, 0, 3) for t in (query, key, value))
+        out, m = ssa_flash_attn_forward(q, k, v, self.softmax_scale, n, b, True)
+        cache.append(k, v)
+        if cache.weights is not None:
+            w = q.shape[2] if window is None else min(window, q.shape[2])
+            if w > 0:
+                cache.add_weights(q[:, :, -w:], m[:, :, -w:], self.softmax_scale, n, b)
+        return out.permute(2, 0, 1, 3).reshape(query.shape[0], query.shape[1], -1)
+
+    def forward_tree(self, query, key, value, cache: SSAKVCache, tree_mask):
+        """One step over a drafted tree of T tokens per sequence.  query [T, B, Hq,
+        D], key/value [T, B, Hkv, D] -> context [T, B, Hq * D]; keys and values are
+        appended to ``cache``, and token i attends the cached prefix and the
+        tokens that ``tree_mask`` ([T, T] or [B, T, T]) gives it.  Then
+        ``cache.accept`` keeps the path that was right."""
+        n, b = self.get_ssa_params()
+        cache.append(key.permute(1, 2, 0, 3), value.permute(1, 2, 0, 3))
+        q = query.permute(1, 2, 0, 3)
+        track = cache.weights is not None
+        ctx = ssa_tree_attention(q, cache.k, cache.v, cache.seqlens, tree_mask, self.softmax_scale, n, b,
+                                 return_m=track)
+        if track:
+            ctx, m = ctx
+            cache._drafted = (q, m, self.softmax_scale, n, b)
+        return ctx.permute(2, 0, 1, 3).reshape(query.shape[0], query.shape[1], -1)

@@ -17,7 +17,9 @@ RoPE, vocab 65536, sequence 4096 (about 1.5 B parameters with an untied output
 layer).  ``train_step`` is one optimizer step under bf16 autocast;
 ``generate`` runs the prompt through the dense forward once and then one
 decode step per token against per-layer KV caches (the reference's loop
-re-runs the whole prefix per token, training/train/train_ssa_triton/generate_triton.py:315-331).
+re-runs the whole prefix per token, training/train/train_ssa_triton/generate_triton.py:315-331);
+with ``keep`` the caches are cut to that many rows by accumulated attention
+weight.  ``generate_drafted`` checks a drafted tree of tokens per step.
 """
 
 from __future__ import annotations
@@ -32,6 +34,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .ssa_attention import SSAAttention, SSAKVCache
+from .ssa_cache_ops import MAX_TREE_NODES, tree_mask_from_parents
 
 
 @dataclass
@@ -206,15 +209,23 @@ class SelfAttention(nn.Module):
         mixed = self.linear_qkv(x).view(S, B, self.ng, (g + 2) * self.hn)
         q, k, v = torch.split(mixed, [g * self.hn, self.hn, self.hn], dim=-1)
         q = q.reshape(S, B, self.np, self.hn)
-        return rope(q, *rot), rope(k, *rot), v
+        if rot[0].shape[0] == S:
+            return rope(q, *rot), rope(k, *rot), v
+        # positions of its own for every token of every sequence: S * B rows of tables
+        q, k = (rope(t.reshape(S * B, 1, -1, self.hn), *rot).view(S, B, -1, self.hn) for t in (q, k))
+        return q, k, v
 
-    def forward(self, x, rot, cache: Optional[SSAKVCache] = None):
+    def forward(self, x, rot, cache: Optional[SSAKVCache] = None, tree_mask=None, window=None):
         """rot = (cos, sin, cos_h, sin_h) from ``SSADecoder.rotary``."""
         q, k, v = self._qkv(x, rot)
         if cache is None:
             ctx = self.core_attention(q, k, v)
+        elif tree_mask is not None:
+            ctx = self.core_attention.forward_tree(q, k, v, cache, tree_mask)
         elif x.shape[0] == 1:
             ctx = self.core_attention.forward_decode(q, k, v, cache)
+        elif cache.weights is not None:
+            ctx = self.core_attention.forward_prompt(q, k, v, cache, window)
         else:  # prompt: dense causal forward, then the keys and values go to the cache
             ctx = self.core_attention(q, k, v)
             cache.append(k.permute(1, 2, 0, 3), v.permute(1, 2, 0, 3))
@@ -384,8 +395,8 @@ class TransformerLayer(nn.Module):
         self.pre_mlp_layernorm = RMSNorm(cfg.hidden_size, cfg.norm_eps, cfg.fused_norm)
         self.mlp = MLP(cfg)
 
-    def forward(self, x, rot, cache=None):
-        x = x + self.self_attention(self.input_layernorm(x), rot, cache)
+    def forward(self, x, rot, cache=None, tree_mask=None, window=None):
+        x = x + self.self_attention(self.input_layernorm(x), rot, cache, tree_mask, window)
         return x + self.mlp(self.pre_mlp_layernorm(x))
 
 
@@ -408,16 +419,27 @@ class SSADecoder(nn.Module):
                 continue
             p.normal_(0.0, out_std if name.endswith(("linear_proj.weight", "linear_fc2.weight")) else std)
 
-    def forward(self, input_ids, caches: Optional[List[SSAKVCache]] = None, start_pos: int = 0):
+    def forward(self, input_ids, caches: Optional[List[SSAKVCache]] = None, start_pos: int = 0, positions=None,
+                tree_mask=None, window: Optional[int] = None):
         """input_ids [B, S] -> logits [S, B, vocab] (Megatron order).  With
         ``caches`` (one per layer) the tokens are positions start_pos .. and
-        their keys / values are appended to the caches."""
+        their keys / values are appended to the caches.  ``positions`` [B, S]
+        gives every token a position of its own instead, and with ``tree_mask``
+        ([S, S] or [B, S, S]) the tokens are a drafted tree behind the cached
+        prefix (``SSAAttention.forward_tree``).  ``window``: how many of a
+        prompt's last tokens add to the weights of a cache that tracks them
+        (None: all)."""
         S = input_ids.shape[1]
         x = self.embedding(input_ids.t())  # [S, B, h]
-        pos = torch.arange(start_pos, start_pos + S, device=input_ids.device)
-        rot = self.rotary(pos)
+        if positions is None:
+            positions = torch.arange(start_pos, start_pos + S, device=input_ids.device)
+        elif positions.shape != input_ids.shape:
+            raise ValueError(f"positions must be [B, S] = {tuple(input_ids.shape)}")
+        else:
+            positions = positions.t().reshape(-1)
+        rot = self.rotary(positions)
         for i, layer in enumerate(self.layers):
-            x = layer(x, rot, None if caches is None else caches[i])
+            x = layer(x, rot, None if caches is None else caches[i], tree_mask, window)
         return self.output_layer(self.final_layernorm(x))
 
     def rotary(self, positions):
@@ -436,28 +458,132 @@ class SSADecoder(nn.Module):
             return FusedCrossEntropy.apply(logits.view(-1, V), labels.t().reshape(-1))
         return F.cross_entropy(logits.float().view(-1, V), labels.t().reshape(-1))
 
-    def new_caches(self, batch: int, capacity: int, dtype=torch.bfloat16) -> List[SSAKVCache]:
+    def new_caches(self, batch: int, capacity: int, dtype=torch.bfloat16,
+                   track_weights: bool = False) -> List[SSAKVCache]:
         dev = self.embedding.weight.device
-        return [SSAKVCache(batch, self.cfg.num_query_groups, capacity, self.cfg.kv_channels, dtype, dev)
+        return [SSAKVCache(batch, self.cfg.num_query_groups, capacity, self.cfg.kv_channels, dtype, dev, track_weights)
                 for _ in range(self.cfg.num_layers)]
 
     @torch.no_grad()
-    def generate(self, input_ids, max_new_tokens: int, dtype=torch.bfloat16):
+    def generate(self, input_ids, max_new_tokens: int, dtype=torch.bfloat16, keep: Optional[int] = None,
+                 sinks: int = 4, recent: int = 32, slack: int = 64, window: Optional[int] = 32):
         """Greedy decoding: the prompt through the dense forward, then one decode
         step per new token.  Returns (tokens [B, P + max_new_tokens], the
-        logits of every generated position [max_new_tokens, B, vocab])."""
+        logits of every generated position [max_new_tokens, B, vocab]).
+
+        With ``keep`` every layer's cache is bounded: when it holds ``slack`` more
+        rows than ``keep`` (and after a longer prompt) it is cut to ``keep`` rows,
+        the first ``sinks``, the last ``recent`` and those that the prompt's last
+        ``window`` tokens (None: all) and every token since paid most attention
+        to.  Tokens keep their positions in the text."""
         B, P = input_ids.shape
-        caches = self.new_caches(B, P + max_new_tokens, dtype)
+        if keep is None:
+            caches = self.new_caches(B, P + max_new_tokens, dtype)
+        else:
+            if keep < 1 or slack < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+                raise ValueError(f"keep must hold sinks + recent and slack be at least 1, got keep={keep} "
+                                 f"sinks={sinks} recent={recent} slack={slack}")
+            caches = self.new_caches(B, max(P, keep + slack), dtype, track_weights=True)
+        held = P  # rows of every cache
         out, steps = input_ids, []
         with torch.autocast("cuda", dtype=dtype):
-            logits = self(input_ids, caches, 0)[-1]
+            logits = self(input_ids, caches, 0, window=window)[-1]
             for t in range(max_new_tokens):
                 steps.append(logits.float())
                 nxt = logits.argmax(-1, keepdim=True)
                 out = torch.cat([out, nxt], dim=1)
                 if t + 1 < max_new_tokens:
+                    if keep is not None and held >= (keep + slack if t else keep + 1):
+                        for cache in caches:
+                            cache.evict(keep, sinks, recent)
+                        held = keep
                     logits = self(nxt, caches, P + t)[-1]
+                    held += 1
         return out, torch.stack(steps)
+
+    @torch.no_grad()
+    def generate_drafted(self, input_ids, max_new_tokens: int, draft, max_nodes: int = 64, dtype=torch.bfloat16):
+        """Greedy decoding where every step checks a drafted tree of tokens.
+
+        ``draft(tokens)`` gets every sequence's tokens so far (a list of B lists) and
+        returns ``(tokens, parents)``, for every sequence the drafted tokens and,
+        of each, the index of its parent among them (before it) or -1 where it
+        follows the last token; at most ``max_nodes`` - 1 of them.  A step runs
+        the last token and the drafted ones as one tree and keeps the longest path
+        on which every token is the one the model picks; the model's pick behind it
+        is the next token.  The result is ``generate``'s (up to logits that are equal
+        within their rounding).  Returns (tokens [B, P + max_new_tokens], steps)."""
+        if not 1 <= max_nodes <= MAX_TREE_NODES:
+            raise ValueError(f"max_nodes must be 1 .. {MAX_TREE_NODES}")
+        B, P = input_ids.shape
+        dev = input_ids.device
+        if max_new_tokens < 1:
+            return input_ids, 0
+        caches = self.new_caches(B, P + max_new_tokens + max_nodes, dtype)
+        text, steps = input_ids.tolist(), 0
+        end = P + max_new_tokens
+        with torch.autocast("cuda", dtype=dtype):
+            first = self(input_ids, caches, 0)[-1].argmax(-1).tolist()
+            for seq, tok in zip(text, first):
+                seq.append(tok)
+            while any(len(seq) < end for seq in text):
+                drafted, above = draft([list(seq) for seq in text])
+                T = 1 + max(len(d) for d in drafted)
+                if len(drafted) != B or len(above) != B or T > max_nodes:
+                    raise ValueError(f"a draft is {B} sequences of at most {max_nodes - 1} tokens and their parents")
+                # node 0 is the last token; short drafts end in nodes that nothing follows
+                nodes = [[seq[-1], *d] + [0] * (T - 1 - len(d)) for seq, d in zip(text, drafted)]
+                parents = [[-1, *(q + 1 for q in a)] + [0] * (T - 1 - len(a)) for a in above]
+                if any(len(d) != len(a) or min(a, default=0) < -1 for d, a in zip(drafted, above)):
+                    raise ValueError("every drafted token needs its parent: an earlier one's index, or -1")
+                mask = tree_mask_from_parents(parents)  # a parent that is not before its child is refused here
+                depth = mask.sum(-1) - 1
+                pos = depth + torch.tensor([[len(seq) - 1] for seq in text])
+                picks = self(torch.tensor(nodes, device=dev), caches, positions=pos.to(dev),
+                             tree_mask=mask.to(dev)).argmax(-1).t().tolist()
+                paths, counts = [], []
+                for i, seq in enumerate(text):
+                    path = [0]
+                    if len(seq) >= end:  # done: nothing stays
+                        paths.append(path)
+                        counts.append(0)
+                        continue
+                    while True:
+                        seq.append(picks[i][path[-1]])
+                        step = [c for c in range(path[-1] + 1, 1 + len(drafted[i]))
+                                if parents[i][c] == path[-1] and nodes[i][c] == seq[-1]]
+                        if not step or len(seq) >= end:
+                            break
+                        path.append(step[0])
+                    paths.append(path)
+                    counts.append(len(path))
+                most = max(map(len, paths))
+                path = torch.tensor([x + [0] * (most - len(x)) for x in paths], dtype=torch.int32, device=dev)
+                count = torch.tensor(counts, dtype=torch.int32, device=dev)
+                for cache in caches:
+                    cache.accept(path, count, T)
+                steps += 1
+        return torch.tensor([seq[:end] for seq in text], device=dev, dtype=input_ids.dtype), steps
+
+
+def lookup_draft(ngram: int = 2, length: int = 8):
+    """A draft for ``SSADecoder.generate_drafted`` that needs no model: the
+    ``length`` tokens that followed the last earlier occurrence of a sequence's
+    last ``ngram`` tokens, as a chain."""
+
+    def draft(texts):
+        tokens, parents = [], []
+        for seq in texts:
+            found, key = [], seq[-ngram:]
+            for at in range(len(seq) - ngram - 1, -1, -1):
+                if seq[at:at + ngram] == key:
+                    found = seq[at + ngram:at + ngram + length]
+                    break
+            tokens.append(found)
+            parents.append(list(range(-1, len(found) - 1)))
+        return tokens, parents
+
+    return draft
 
 
 def train_step(model: SSADecoder, optimizer: torch.optim.Optimizer, input_ids, labels, dtype=torch.bfloat16):

@@ -156,12 +156,15 @@ def _check_seen(dev, q, k, v, lens, mask):
     return r
 
 
-@pytest.mark.parametrize("n", [0.0, -3.5, 5.0])
+@pytest.mark.parametrize("n,b", [(0.0, 0.8), (-3.5, 0.8), (5.0, 0.8), (1.5, 0.0), (-302.0, 0.8), (1e-30, 0.8)])
 @pytest.mark.parametrize("T", [9, 40, 100])
-def test_tree_scalars(gpu, n, T):
-    _say(f"tree n={n} T={T}")
+def test_tree_and_weights_scalars(gpu, n, b, T):
+    """n of both signs, 0 and tiny, b = 0; queries whose exponents lie far below 0."""
+    _say(f"tree and weights n={n} b={b} T={T}")
     k, v, g = _caches(gpu, 1, 2, 400, 64, BF16, seed=7)
-    _check_tree(gpu, _randn((1, 4, T, 64), g, BF16, gpu), k, v, [400], _random_tree(T, 3), n=n)
+    q = _randn((1, 4, T, 64), g, BF16, gpu)
+    _check_tree(gpu, q, k, v, [400], _random_tree(T, 3), n=n, b=b)
+    _check_weights(gpu, q, k, [400], n=n, b=b)
 
 
 @pytest.mark.parametrize("T", [5, 30, 70])
