@@ -168,7 +168,7 @@ int32_t ssa_key_weights(const ssa_key_weights_args* a, void* stream) {
     return SSA_ERR_ALIGNMENT;
   ssa::KeyWeightsParams p{};
   p.chunks = ssa::weights_chunks(a->batch, a->heads_q, a->heads_kv, a->capacity, a->queries);
-  p.chunk_rows = ssa::weights_chunk_rows(static_cast<int64_t>(a->heads_q / a->heads_kv) * a->queries, p.chunks);
+  p.chunk_rows = ssa::weights_chunk_rows(a->batch, a->heads_q, a->heads_kv, a->capacity, a->queries);
   if (p.chunks > 1) {
     if (a->workspace == nullptr) return SSA_ERR_NULL_POINTER;
     if (!aligned16(a->workspace)) return SSA_ERR_ALIGNMENT;

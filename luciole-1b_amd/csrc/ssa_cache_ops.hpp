@@ -103,19 +103,21 @@ inline int tree_splits(int B, int Hq, int Hkv, int cap, int T, int requested) {
 // Key weights of more than 32 rows: rows of a stage and keys of a workgroup.
 constexpr int kWeightsStage = 128;
 constexpr int kWeightsKeys = 128;
-// Chunks of the rows: about 2048 workgroups in all, so that those of many rows
-// and of few even out, of 1024 rows at least.
-inline int weights_chunks(int B, int Hq, int Hkv, int cap, int T) {
+// Rows of a chunk (whole stages): about 2048 workgroups in all, so that those of
+// many rows and of few even out, of 1024 rows at least.
+inline int weights_chunk_rows(int B, int Hq, int Hkv, int cap, int T) {
   const int64_t rows = static_cast<int64_t>(Hq / Hkv) * T;
-  if (rows <= 32) return 1;
   const int64_t blocks = static_cast<int64_t>(B) * Hkv * ((cap + kWeightsKeys - 1) / kWeightsKeys);
   const int64_t want = 2048 / blocks, most = rows / 1024;
-  const int64_t n = want < most ? want : most;
-  return static_cast<int>(n < 1 ? 1 : n);
-}
-inline int weights_chunk_rows(int64_t rows, int chunks) {
-  const int64_t per = (rows + chunks - 1) / chunks;
+  int64_t n = want < most ? want : most;
+  if (n < 1 || rows <= 32) n = 1;
+  const int64_t per = (rows + n - 1) / n;
   return static_cast<int>((per + kWeightsStage - 1) / kWeightsStage * kWeightsStage);
+}
+// ... and the chunks that hold rows: every one is written, every one is read.
+inline int weights_chunks(int B, int Hq, int Hkv, int cap, int T) {
+  const int64_t rows = static_cast<int64_t>(Hq / Hkv) * T, per = weights_chunk_rows(B, Hq, Hkv, cap, T);
+  return static_cast<int>((rows + per - 1) / per);
 }
 
 hipError_t launch_tree(const TreeParams& p, int dtype, int D, hipStream_t stream);

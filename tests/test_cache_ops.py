@@ -113,6 +113,18 @@ def test_weights_workspace():
     assert _lib.lib().ssa_key_weights(ctypes.byref(a), None) == A
 
 
+@pytest.mark.parametrize("heads,T,cap", [(32, 1200, 1280), (32, 4000, 4096), (24, 3000, 3000), (7, 1000, 1000)])
+def test_weights_chunks_all_hold_rows(heads, T, cap):
+    """No chunk of the rows is empty: its part of the workspace would be added
+    up without having been written."""
+    chunks = _lib.lib().ssa_key_weights_workspace_bytes(1, heads, 1, cap, T) // (cap * 4)
+    rows = heads * T
+    # chunks of one length that is whole stages of 128 rows, 1024 rows or more: some
+    # length makes that many of them without an empty one
+    assert chunks >= 2 and rows // chunks >= 1000
+    assert any((rows + per - 1) // per == chunks for per in range(1024, rows + 128, 128))
+
+
 def test_tree_splits_and_workspace():
     lib = _lib.lib()
     n, w = lib.ssa_tree_num_splits, lib.ssa_tree_workspace_bytes

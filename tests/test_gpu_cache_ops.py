@@ -328,6 +328,18 @@ def test_weights_strides_and_sums(gpu):
     assert torch.allclose(w.sum(-1), torch.full((2, 2), 2.0 * L, device=gpu), rtol=2.0 ** -12)
 
 
+def test_weights_of_chunks_that_do_not_divide(gpu):
+    """Rows split into chunks that whole stages make longer than an even share;
+    the workspace comes from memory that held NaN."""
+    B, Hq, Hk, cap, T, D = 1, 32, 1, 1280, 1200, 32
+    _say("weights of 38400 rows in chunks of 1152")
+    k, _, g = _caches(gpu, B, Hk, cap, D, BF16, seed=11)
+    q = _randn((B, Hq, T, D), g, BF16, gpu)
+    for size in (37 * cap, 34 * cap):
+        torch.full((size,), math.nan, device=gpu)  # freed at once, for the next of its size
+    _check_weights(gpu, q, k, [1250])
+
+
 # ------------------------------------------------------------------------ evict
 def _check_evict(dev, lens, weights, keep, sinks, recent, D=64, dtype=BF16, layout="bhsd"):
     from SSA import ssa_cache_evict
