@@ -76,8 +76,10 @@ bool tree_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t cap, int32_t T, int32_t
 }
 
 bool weights_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t cap, int32_t T) {
-  // at most 2^28 * 4 workgroups
-  return cache_ok(B, Hkv, cap) && rows_ok(B, Hq, Hkv, T) && T <= cap;
+  // a tile of 128 keys may end up to 127 behind the last query, and the first row
+  // that would see its last key is counted with int32 too
+  return cache_ok(B, Hkv, cap) && rows_ok(B, Hq, Hkv, T) && T <= cap &&
+         static_cast<int64_t>(Hq / Hkv) * (static_cast<int64_t>(T) + 128) < (1ll << 31);
 }
 
 int64_t tree_ml_floats(int64_t recs) { return (2 * recs + 3) & ~static_cast<int64_t>(3); }

@@ -125,6 +125,17 @@ def test_weights_chunks_all_hold_rows(heads, T, cap):
     assert any((rows + per - 1) // per == chunks for per in range(1024, rows + 128, 128))
 
 
+def test_weights_of_groups_past_int32():
+    """The first row that sees the last key of a tile is counted with 32 bits: up to
+    128 queries past the last, times the heads of a group."""
+    f = _lib.lib().ssa_key_weights
+    q = _lib.Tensor4(FAKE, 0, 0, 64)
+    for heads, queries, status in [(1 << 29, 1, S), (1 << 24, 1, S), (1 << 23, 128, S), (1 << 23, 64, N)]:
+        a = _weights(batch=1, heads_q=heads, heads_kv=1, queries=queries, q=q, m=None)
+        assert f(ctypes.byref(a), None) == status
+        assert status == N or _lib.lib().ssa_key_weights_workspace_bytes(1, heads, 1, 4096, queries) == 0
+
+
 def test_tree_splits_and_workspace():
     lib = _lib.lib()
     n, w = lib.ssa_tree_num_splits, lib.ssa_tree_workspace_bytes
