@@ -104,16 +104,17 @@ class SSAKVCache:
         ``accepted[b]`` nodes of ``path[b]``, in that order
         (``ssa_cache_accept``).  A tracking cache gains the attention that the
         accepted tokens paid."""
-        drafted, self._drafted = self._drafted, None
-        path = torch.as_tensor(path, device=self.k.device).to(torch.int32)
-        accepted = torch.as_tensor(accepted, device=self.k.device).to(torch.int32)
+        drafted = self._drafted
+        if drafted is not None and drafted[0].shape[2] != nodes:
+            raise ValueError(f"the last tree had {drafted[0].shape[2]} nodes, not {nodes}")
+        path = torch.as_tensor(path, device=self.k.device)
+        accepted = torch.as_tensor(accepted, device=self.k.device)
         held = self.seqlens >= nodes
         self.seqlens.copy_(ssa_cache_accept(self.k, self.v, self.seqlens, path, accepted, nodes))
+        self._drafted = None
         if self.weights is None or drafted is None:
             return
         q, m, scale, n, b = drafted
-        if q.shape[2] != nodes:
-            raise ValueError(f"the last tree had {q.shape[2]} nodes, not {nodes}")
         # the path's queries at the end of the sequence, rows that were not accepted before them
         depth = path.shape[1]
         count = torch.where(held, accepted.clamp(0, depth), torch.zeros_like(accepted)).long()

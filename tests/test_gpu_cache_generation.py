@@ -160,6 +160,29 @@ def test_refusals_on_the_gpu(gpu):
 
 
 # ------------------------------------------------------------------ the decoder
+def test_accept_of_another_tree_leaves_the_cache(gpu):
+    """A number of nodes that is not the last tree's is refused before anything moves."""
+    from SSA import SSAAttention, SSAKVCache
+
+    _say("accept with another number of nodes")
+    mod = SSAAttention(4, 2, 64).to(gpu).eval()
+    cache = SSAKVCache(1, 2, 64, 64, BF16, gpu, track_weights=True)
+    with torch.no_grad():
+        mod.forward_prompt(*_qkv(gpu, 20, 1, 4, 2, 64, 3), cache)
+        mod.forward_tree(*_qkv(gpu, 5, 1, 4, 2, 64, 4), cache, torch.ones(5, 5, device=gpu).tril())
+    before = [t.clone() for t in (cache.k, cache.v, cache.seqlens, cache.weights)]
+    with pytest.raises(ValueError):
+        cache.accept(torch.tensor([[0, 2]], device=gpu), torch.tensor([2], device=gpu), 6)
+    assert all(torch.equal(a, b) for a, b in zip(before, (cache.k, cache.v, cache.seqlens, cache.weights)))
+    with pytest.raises(ValueError):
+        cache.accept(torch.tensor([[0.0, 2.5]], device=gpu), torch.tensor([2], device=gpu), 5)
+    cache.accept(torch.tensor([[0, 2]], device=gpu), torch.tensor([2], device=gpu), 5)
+    assert cache.seqlens.tolist() == [22]
+    # 4 heads, 22 tokens, at most 1 each: node 2 also paid node 1, which did not stay
+    # (the normalisers are fp32 sums, each p within 2^-12 of its own)
+    assert float(cache.weights.sum()) <= 4 * 22 * (1 + 2.0 ** -12)
+
+
 def _decoder(gpu, **kw):
     from SSA.ssa_decoder import SSADecoder, SSADecoderConfig
 
