@@ -528,15 +528,8 @@ class SSADecoder(nn.Module):
                 seq.append(tok)
             while any(len(seq) < end for seq in text):
                 drafted, above = draft([list(seq) for seq in text])
-                T = 1 + max(len(d) for d in drafted)
-                if len(drafted) != B or len(above) != B or T > max_nodes:
-                    raise ValueError(f"a draft is {B} sequences of at most {max_nodes - 1} tokens and their parents")
-                # node 0 is the last token; short drafts end in nodes that nothing follows
-                nodes = [[seq[-1], *d] + [0] * (T - 1 - len(d)) for seq, d in zip(text, drafted)]
-                parents = [[-1, *(q + 1 for q in a)] + [0] * (T - 1 - len(a)) for a in above]
-                if any(len(d) != len(a) or min(a, default=0) < -1 for d, a in zip(drafted, above)):
-                    raise ValueError("every drafted token needs its parent: an earlier one's index, or -1")
-                mask = tree_mask_from_parents(parents)  # a parent that is not before its child is refused here
+                nodes, parents, mask = drafted_tree(text, drafted, above, max_nodes, self.cfg.vocab_size)
+                T = len(nodes[0])
                 depth = mask.sum(-1) - 1
                 pos = depth + torch.tensor([[len(seq) - 1] for seq in text])
                 picks = self(torch.tensor(nodes, device=dev), caches, positions=pos.to(dev),
@@ -564,6 +557,26 @@ class SSADecoder(nn.Module):
                     cache.accept(path, count, T)
                 steps += 1
         return torch.tensor([seq[:end] for seq in text], device=dev, dtype=input_ids.dtype), steps
+
+
+def drafted_tree(texts, drafted, above, max_nodes: int, vocab: int):
+    """The trees of a step of ``generate_drafted``: every sequence's last token as
+    node 0, then its drafted tokens, and nodes that nothing follows up to the
+    longest draft's length.  Returns (tokens, parents, mask ``[B, T, T]``) with the
+    parents as node indices; drafts that are no such trees, or whose tokens are not in
+    the vocabulary, are refused."""
+    B = len(texts)
+    if len(drafted) != B or len(above) != B or any(len(d) >= max_nodes for d in drafted):
+        raise ValueError(f"a draft is {B} sequences of at most {max_nodes - 1} tokens and their parents")
+    drafted, above = [[int(x) for x in d] for d in drafted], [[int(x) for x in a] for a in above]
+    if any(len(d) != len(a) or min(a, default=0) < -1 for d, a in zip(drafted, above)):
+        raise ValueError("every drafted token needs its parent: an earlier one's index, or -1")
+    if any(not 0 <= x < vocab for d in drafted for x in d):
+        raise ValueError(f"drafted tokens must be 0 .. {vocab - 1}")
+    T = 1 + max(len(d) for d in drafted)
+    nodes = [[seq[-1], *d] + [0] * (T - 1 - len(d)) for seq, d in zip(texts, drafted)]
+    parents = [[-1, *(q + 1 for q in a)] + [0] * (T - 1 - len(a)) for a in above]
+    return nodes, parents, tree_mask_from_parents(parents)  # refuses a parent that is not before its child
 
 
 def lookup_draft(ngram: int = 2, length: int = 8):

@@ -220,6 +220,24 @@ def test_lookup_draft():
     assert parents == [[-1, 0, 1], [], [-1], []]
 
 
+def test_drafted_tree():
+    """Node 0 is the last token; drafts that are no trees, too long ones and tokens
+    outside the vocabulary (whose embedding would be read past the table) are refused."""
+    from SSA.ssa_decoder import drafted_tree
+
+    texts = [[3, 1], [4]]
+    nodes, parents, mask = drafted_tree(texts, [[5, 6, 7], torch.tensor([9])], [[-1, 0, -1], [-1]], 4, 10)
+    assert nodes == [[1, 5, 6, 7], [4, 9, 0, 0]] and parents == [[-1, 0, 1, 0], [-1, 0, 0, 0]]
+    assert mask[0].tolist() == [[True, False, False, False], [True, True, False, False], [True, True, True, False],
+                                [True, False, False, True]]
+    assert drafted_tree(texts, [[], []], [[], []], 1, 10)[0] == [[1], [4]]
+    for bad in (([[10], []], [[-1], []]), ([[-1], []], [[-1], []]), ([[1, 2, 3, 4], []], [[-1, 0, 1, 2], []]),
+                ([[1], []], [[], []]), ([[1], []], [[0], []]), ([[1], []], [[-2], []]), ([[1]], [[-1]]),
+                ([[1, 2], []], [[-1, 1], []])):
+        with pytest.raises(ValueError):
+            drafted_tree(texts, *bad, 4, 10)
+
+
 def test_generate_refuses_budgets_that_cannot_hold():
     from SSA.ssa_decoder import SSADecoder, SSADecoderConfig
 
