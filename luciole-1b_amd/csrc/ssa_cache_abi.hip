@@ -71,8 +71,8 @@ bool rows_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t T) {
 bool tree_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t cap, int32_t T, int32_t requested) {
   if (!cache_ok(B, Hkv, cap) || !rows_ok(B, Hq, Hkv, T) || T > SSA_TREE_MAX_NODES || requested < 0) return false;
   // workgroups over all splits, and the merge's threads, stay below 2^30
-  const int64_t splits = ssa::tree_splits(B, Hq, Hkv, cap, T, requested);
-  return ssa::tree_units(B, Hq, Hkv, T) * splits < (1ll << 30);
+  const ssa::TreePlan plan = ssa::tree_plan(B, Hq, Hkv, cap, T, requested);
+  return plan.units * plan.splits < (1ll << 30);
 }
 
 bool weights_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t cap, int32_t T) {
@@ -95,14 +95,14 @@ extern "C" {
 int32_t ssa_tree_num_splits(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t capacity, int32_t nodes,
                             int32_t requested) {
   if (!tree_ok(batch, heads_q, heads_kv, capacity, nodes, requested)) return 0;
-  return ssa::tree_splits(batch, heads_q, heads_kv, capacity, nodes, requested);
+  return ssa::tree_plan(batch, heads_q, heads_kv, capacity, nodes, requested).splits;
 }
 
 int64_t ssa_tree_workspace_bytes(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t capacity,
                                  int32_t head_dim, int32_t nodes, int32_t requested) {
   if (!tree_ok(batch, heads_q, heads_kv, capacity, nodes, requested)) return 0;
   if (head_dim != 32 && head_dim != 64 && head_dim != 128) return 0;
-  const int64_t splits = ssa::tree_splits(batch, heads_q, heads_kv, capacity, nodes, requested);
+  const int64_t splits = ssa::tree_plan(batch, heads_q, heads_kv, capacity, nodes, requested).splits;
   if (splits <= 1) return 0;
   const int64_t recs = static_cast<int64_t>(batch) * heads_q * nodes * splits;
   return (tree_ml_floats(recs) + recs * head_dim) * 4;
@@ -120,8 +120,11 @@ int32_t ssa_tree_attention(const ssa_tree_args* a, void* stream) {
     return SSA_ERR_NULL_POINTER;
   if (a->mask_stride_b < 0) return SSA_ERR_ALIGNMENT;
   ssa::TreeParams p{};
-  p.splits = ssa::tree_splits(a->batch, a->heads_q, a->heads_kv, a->capacity, a->nodes, a->num_splits);
-  p.split_keys = ssa::tree_split_keys(a->batch, a->heads_q, a->heads_kv, a->capacity, a->nodes, a->num_splits);
+  const ssa::TreePlan plan =
+      ssa::tree_plan(a->batch, a->heads_q, a->heads_kv, a->capacity, a->nodes, a->num_splits);
+  p.splits = plan.splits;
+  p.split_keys = plan.split_keys;
+  p.rows = plan.rows;
   if (p.splits > 1) {
     if (a->workspace == nullptr) return SSA_ERR_NULL_POINTER;
     if (!aligned16(a->workspace)) return SSA_ERR_ALIGNMENT;

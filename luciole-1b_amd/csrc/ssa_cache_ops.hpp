@@ -2,6 +2,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <stdint.h>
 
 #include "ssa_common.hpp"
 
@@ -21,6 +22,7 @@ struct TreeParams {
   float* ws_acc;  // [B * Hq * T * splits][D]
   int B, Hq, Hkv, cap, T;
   int splits, split_keys;  // split s: keys s * split_keys ..
+  int rows;                // rows of a workgroup (TreePlan)
   float scale;
 };
 
@@ -58,59 +60,81 @@ struct AcceptParams {
   int B, Hkv, cap, D, T, depth;
 };
 
-// q rows that one workgroup of the tree kernels covers.
-inline int tree_rows_per_block(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+// How a tree launch is cut: rows of a group per workgroup, row blocks x kv-heads x
+// sequences, keys of a split (a multiple of 256, the steps of every kernel).
+struct TreePlan {
+  int rows;
+  int64_t units;
+  int split_keys, splits;
+};
 
-// Workgroups of a tree launch per split, or -1 beyond 2^30.
-inline int64_t tree_units(int B, int Hq, int Hkv, int T) {
-  const int64_t rows = static_cast<int64_t>(Hq / Hkv) * T;
-  const int per = tree_rows_per_block(rows);
-  return static_cast<int64_t>(B) * Hkv * ((rows + per - 1) / per);
-}
-
-// Keys of a split (a multiple of 256, the steps of every kernel) for a wanted
-// number of splits.  The default takes the number that makes
-//   rounds of one workgroup a CU * (keys of a split + what one costs beside them)
-// least: a workgroup's start, end and share of the merge take as long as about
-// 400 keys (measured: 8 to 12 us, 16 to 32 ns a key).
-constexpr int kTreeStep = 256, kTreeOverhead = 400, kCUs = 256;
-inline int tree_split_keys(int B, int Hq, int Hkv, int cap, int T, int requested) {
-  const auto keys_of = [cap](int64_t splits) {
-    const int64_t keys = (cap + splits - 1) / splits;
-    return (keys + kTreeStep - 1) / kTreeStep * kTreeStep;
+// The plan of least estimated time, ns:
+//   rounds of one workgroup a CU * (start and end + keys of a split * time of one)
+//   + the merge's launch, if any + the masked keys of the last split
+// The constants were fitted to 2300 measured calls on caches read from HBM: 28
+// shapes (1 to 64 sequences, 8 to 8192 rows of a group, 1000 to 65536 keys) at all
+// head dims, in every form and with 1 to 64 splits.  The plans chosen take 2 %
+// longer than each shape's best, 12 % at most; workgroups of as many rows as there are
+// take 10 and 136 %.  So few keys or workgroups go to 32 rows (2 x 24/8 heads x
+// 1000 x 32, 61 nodes: 9.9 us a call, 17.6 with 256 rows), most others to 64 (1 x 8 x
+// 16384 x 64, 1024 nodes: 106, 32 rows 116, 128 rows 138, 256 rows 207, whose last
+// split holds all masked keys), long caches of many rows to 256 (1 x 32/8 x 65536 x
+// 64, 64 nodes: 73.8, 128 rows 77.5; head dim 128: 120, 128 rows 128, 64 rows 141).
+constexpr int kTreeStep = 256, kCUs = 256;
+inline TreePlan tree_plan(int B, int Hq, int Hkv, int cap, int T, int requested) {
+  struct Form {
+    int rows;
+    int64_t start, key;  // ns; tenths of ns
   };
-  if (requested > 0) return static_cast<int>(keys_of(requested));
-  const int64_t units = tree_units(B, Hq, Hkv, T);
-  int64_t most = 2 * kCUs / units;
-  if (most < 4) most = 4;
-  if (most > (cap + kTreeStep - 1) / kTreeStep) most = (cap + kTreeStep - 1) / kTreeStep;
-  int64_t best = keys_of(1), least = (units + kCUs - 1) / kCUs * (best + kTreeOverhead);
-  for (int64_t s = 2; s <= most; ++s) {
-    const int64_t keys = keys_of(s), n = (cap + keys - 1) / keys;
-    const int64_t cost = (units * n + kCUs - 1) / kCUs * (keys + kTreeOverhead);
-    if (cost < least) {
-      least = cost;
-      best = keys;
+  constexpr Form kForms[] = {{32, 7000, 80}, {64, 9000, 110}, {128, 12000, 195}, {256, 12000, 350}};
+  constexpr int64_t kMerge = 4500;
+  const int64_t rows = static_cast<int64_t>(Hq / Hkv) * T;
+  const int64_t steps = (static_cast<int64_t>(cap) + kTreeStep - 1) / kTreeStep;
+  TreePlan best{};
+  int64_t least = INT64_MAX;
+  for (const Form& f : kForms) {
+    const int64_t units = static_cast<int64_t>(B) * Hkv * ((rows + f.rows - 1) / f.rows);
+    int64_t most = 2 * kCUs / units;
+    if (most < 4) most = 4;
+    if (requested > 0) most = requested;
+    if (most > steps) most = steps;
+    for (int64_t s = requested > 0 ? most : 1; s <= most; ++s) {
+      const int64_t keys = (steps + s - 1) / s * kTreeStep, n = (cap + keys - 1) / keys;
+      const int64_t masked = T < keys ? T : keys;
+      const int64_t cost = (units * n + kCUs - 1) / kCUs * (f.start + keys * f.key / 10) + (n > 1 ? kMerge : 0) +
+                           3 * masked * f.rows / 10;
+      if (cost < least) {
+        least = cost;
+        best = TreePlan{f.rows, units, static_cast<int>(keys), static_cast<int>(n)};
+      }
     }
   }
-  return static_cast<int>(best);
-}
-inline int tree_splits(int B, int Hq, int Hkv, int cap, int T, int requested) {
-  const int keys = tree_split_keys(B, Hq, Hkv, cap, T, requested);
-  return static_cast<int>((static_cast<int64_t>(cap) + keys - 1) / keys);
+  return best;
 }
 
-// Key weights of more than 32 rows: rows of a stage and keys of a workgroup.
-constexpr int kWeightsStage = 128;
+// Key weights: keys of a workgroup, and rows of a stage (whole stages make a chunk).
+constexpr int kWeightsStage = 64;
 constexpr int kWeightsKeys = 128;
+inline int64_t weights_blocks(int B, int Hkv, int cap) {
+  return static_cast<int64_t>(B) * Hkv * ((static_cast<int64_t>(cap) + kWeightsKeys - 1) / kWeightsKeys);
+}
+// One wave of rows (32 a stage) or two (64).  One, whose workgroups are small and many to
+// a CU, up to 64 rows (4 x 16 x 8192 x 128, 48 rows: 31.6 us, two 47.6) and, where
+// there are 8 workgroups a CU, up to 512 (192 rows 55 and 72, head dim 64 40 and
+// 44); two beyond (768 rows at head dim 64: 117, one 121) and where few
+// workgroups are to hide a row's latency (1 x 32/8 x 4096 x 64, 192 rows: 6.5, one
+// 8.4; 768 rows 15.4 and 25.2).
+inline bool weights_one_wave(int64_t rows, int64_t blocks) { return rows <= 64 || (rows <= 512 && blocks >= 8 * 256); }
 // Rows of a chunk (whole stages): about 2048 workgroups in all, so that those of
-// many rows and of few even out, of 1024 rows at least.
+// many rows and of few even out (1 x 32/8 x 4096 x 64, 4096 queries: 155 us in
+// one chunk, 107 in 8), of 512 rows at least (1 x 8 x 2048 x 64, 1200 rows: 21.9 in
+// one, 16.0 in two, the join's launch included; 256 rows a chunk cost 1 x 32/8 x
+// 4096 x 128, 1536 rows, 37.8 for 33.2).
 inline int weights_chunk_rows(int B, int Hq, int Hkv, int cap, int T) {
   const int64_t rows = static_cast<int64_t>(Hq / Hkv) * T;
-  const int64_t blocks = static_cast<int64_t>(B) * Hkv * ((cap + kWeightsKeys - 1) / kWeightsKeys);
-  const int64_t want = 2048 / blocks, most = rows / 1024;
+  const int64_t want = 2048 / weights_blocks(B, Hkv, cap), most = rows / 512;
   int64_t n = want < most ? want : most;
-  if (n < 1 || rows <= 32) n = 1;
+  if (n < 1) n = 1;
   const int64_t per = (rows + n - 1) / n;
   return static_cast<int>((per + kWeightsStage - 1) / kWeightsStage * kWeightsStage);
 }

@@ -10,10 +10,20 @@
 //
 // The G heads of a group and their T queries are rows r = t * G + head, so the
 // causal mask only bounds the first row of a workgroup's keys and the rows
-// near it.  A workgroup is KW key waves of 32 NK keys by RW row waves of 32
-// rows; Q rows pass through LDS in stages of 32 RW rows, two in flight.  Many
-// rows are split over workgroups in chunks, whose sums a second kernel adds up
-// in their order.
+// near it.  A workgroup is KW key waves of 32 keys by RW row waves of 32 rows; Q
+// rows pass through LDS in stages of 32 RW rows, two in flight.  Many rows are
+// split over workgroups in chunks, whose sums a second kernel adds up in their
+// order.
+//
+// With few rows the stream of K is the bound: 16 x 32/8 heads x 4096 x 64 with one
+// query takes 14.4 us (67 MB of K and 8.4 of weights, 5.2 TB/s), 4 x 16 x 8192 x 128
+// with 32 queries 23.4 (4.5 TB/s of K).  With many it is the transform, one log2
+// and one exp2 a pair, 768 cycles for 32 x 32 pairs on one SIMD, beside which the
+// product (256 at D = 64) is hidden: 1 x 32/8 x 4096 x 64 with 4096 queries takes
+// 103 us and 4 for the join, of 93 to 96 for the transforms alone at the 2.1 GHz
+// that the GPU holds then.  Two groups of 32 keys a wave, so that an operand read
+// from LDS serves two products, took as long there (106 and 107 us) and 1.1 to 1.4
+// times as long at D = 128, where their registers halve the waves of a SIMD.
 #include "ssa_cache_ops.hpp"
 #include "ssa_common.hpp"
 #include "ssa_launch.hpp"
@@ -23,10 +33,10 @@ namespace ssa {
 
 namespace {
 
-template <int D, int KW, int RW, int NK>
+template <int D, int KW, int RW>
 struct WeightsCfg {
   static constexpr int NW = KW * RW;
-  static constexpr int KEYS = 32 * KW * NK;
+  static constexpr int KEYS = 32 * KW;
   static constexpr int ROWS = 32 * RW;              // rows of a stage
   static constexpr int QB = ROWS * D * 2;           // bytes of its Q rows
   static constexpr int PIECES = BlockLayout<D>::IPB;  // 1 KB pieces of a 32-row block
@@ -41,9 +51,9 @@ __device__ __forceinline__ int first_row(int key, int first, int G) { return key
 
 }  // namespace
 
-template <typename T, int D, int KW, int RW, int NK>
+template <typename T, int D, int KW, int RW>
 __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsParams p, int ntiles, int nblocks) {
-  using C = WeightsCfg<D, KW, RW, NK>;
+  using C = WeightsCfg<D, KW, RW>;
   typedef typename Vec8<T>::type v8;
   constexpr int ND16 = D / 16;
   static_assert(KW % 2 == 0, "one piece parity per wave");
@@ -51,7 +61,7 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
   __shared__ __attribute__((aligned(16))) float ms[2][C::ROWS];  // m of the stage's rows
   __shared__ __attribute__((aligned(16))) int ps[2][C::ROWS];    // and their positions; -1: adds nothing
   __shared__ int odd[2][RW];  // a row of the block adds nothing
-  __shared__ float part[C::NW][32 * NK];
+  __shared__ float part[C::NW][32];
 
   const int block = folded_block();
   if (block >= nblocks) return;
@@ -76,11 +86,11 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
   const int kw = wave / RW, rw = wave - kw * RW;
   const int l32 = lane & 31, hh = lane >> 5;
   const float n = *p.n_ptr, c = p.scale * *p.b_ptr;
-  const int kbase = key0 + 32 * NK * kw;  // this wave's keys
+  const int kbase = key0 + 32 * kw;  // this wave's keys
 
   const int nst = (R - rstart + C::ROWS - 1) / C::ROWS;
   // rows of whole blocks that see every key of the wave
-  const int rall = first_row(kbase + 32 * NK - 1, first, G);
+  const int rall = first_row(kbase + 31, first, G);
 
   // the row of its block that this lane's loads fetch, as (query, head), moved
   // on by one stage at a time
@@ -121,17 +131,14 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
   };
   issue(0);
 
-  v8 kf[NK][ND16];
+  v8 kf[ND16];
+  const int key = kbase + l32;  // this lane's
+  {
+    const T* src = static_cast<const T*>(p.k.ptr) + b * p.k.sb + hk * p.k.sh + min(key, L - 1) * p.k.ss + 8 * hh;
 #pragma unroll
-  for (int k = 0; k < NK; ++k) {
-    const int row = min(kbase + 32 * k + l32, L - 1);
-    const T* src = static_cast<const T*>(p.k.ptr) + b * p.k.sb + hk * p.k.sh + row * p.k.ss + 8 * hh;
-#pragma unroll
-    for (int ds = 0; ds < ND16; ++ds) kf[k][ds] = load16<v8>(src + ds * 16);
+    for (int ds = 0; ds < ND16; ++ds) kf[ds] = load16<v8>(src + ds * 16);
   }
-  float sum[NK];
-#pragma unroll
-  for (int k = 0; k < NK; ++k) sum[k] = 0.f;
+  float sum = 0.f;
   const RowBase<D> rb(l32, hh);
 
   for (int i = 0; i < nst; ++i) {
@@ -149,15 +156,9 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
     const int row0 = rstart + i * C::ROWS + 32 * rw;
     if (row0 >= R) continue;
     const RowBase<D> qr = at_tile(rb, lds0 + (i & 1) * C::QB + rw * BlockLayout<D>::BLOCK);
-    f32x16 s[NK];
+    f32x16 s = f32x16{};
 #pragma unroll
-    for (int k = 0; k < NK; ++k) s[k] = f32x16{};
-#pragma unroll
-    for (int ds = 0; ds < ND16; ++ds) {
-      const v8 qf = tile_read_row<D, v8>(qr, 0, ds);
-#pragma unroll
-      for (int k = 0; k < NK; ++k) s[k] = mfma32(qf, kf[k][ds], s[k]);
-    }
+    for (int ds = 0; ds < ND16; ++ds) s = mfma32(tile_read_row<D, v8>(qr, 0, ds), kf[ds], s);
     // every row of the block sees every key of the wave, but near the diagonal
     const bool all = row0 >= rall && !odd[i & 1][rw];
     if (all) {
@@ -166,11 +167,8 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
         const f32x4_t m4 = *reinterpret_cast<const f32x4_t*>(&ms[i & 1][32 * rw + 8 * j + 4 * hh]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-#pragma unroll
-          for (int k = 0; k < NK; ++k) {
-            const float x = s[k][4 * j + e];
-            sum[k] += fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -m4[e]));
-          }
+          const float x = s[4 * j + e];
+          sum += fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -m4[e]));
         }
       }
     } else {
@@ -180,37 +178,30 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
         for (int e = 0; e < 4; ++e) {
           const float m = ms[i & 1][32 * rw + 8 * j + 4 * hh + e];
           const int pos = ps[i & 1][32 * rw + 8 * j + 4 * hh + e];
-#pragma unroll
-          for (int k = 0; k < NK; ++k) {
-            const float x = s[k][4 * j + e];
-            const float pr = fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -m));
-            sum[k] += pos >= kbase + 32 * k + l32 ? pr : 0.f;
-          }
+          const float x = s[4 * j + e];
+          const float pr = fast_exp2(fmaf(n, copysignf(fast_log2(fmaf(c, fabsf(x), 1.f)), x), -m));
+          sum += pos >= key ? pr : 0.f;
         }
       }
     }
   }
-#pragma unroll
-  for (int k = 0; k < NK; ++k) {
-    const float both = pair_sum(sum[k]);
-    if (hh == 0) part[wave][32 * k + l32] = both;
-  }
+  const float both = pair_sum(sum);
+  if (hh == 0) part[wave][l32] = both;
   __syncthreads();
   float* w = p.chunks == 1 ? p.w + b * p.w_sb + hk * p.w_sh
                            : p.ws + (static_cast<int64_t>(chunk) * nbh + bh) * p.cap;
   for (int e = tid; e < C::KEYS; e += C::NW * 64) {
-    const int key = key0 + e;
-    if (key >= L) break;
-    const int k_wave = e / (32 * NK), at = e - k_wave * 32 * NK;
+    const int at = key0 + e;
+    if (at >= L) break;
     float total = 0.f;
 #pragma unroll
-    for (int r = 0; r < RW; ++r) total += part[k_wave * RW + r][at];
-    w[key] = p.chunks == 1 ? w[key] + total : total;
+    for (int r = 0; r < RW; ++r) total += part[e / 32 * RW + r][e % 32];
+    w[at] = p.chunks == 1 ? w[at] + total : total;
   }
 }
 
-// The chunks' sums of each key, in order.  KEYS, ROWS: those of the kernel that made them.
-template <int KEYS, int ROWS>
+// The chunks' sums of each key, in order: a stream of [chunks][keys] floats, 4.2 us
+// for 8 chunks of 32768 keys, as long as a launch takes.
 __global__ __launch_bounds__(256) void key_weights_join_kernel(KeyWeightsParams p, int blocks_per_head, int nblocks) {
   const int block = folded_block();
   if (block >= nblocks) return;
@@ -218,7 +209,7 @@ __global__ __launch_bounds__(256) void key_weights_join_kernel(KeyWeightsParams 
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int L = clamped_length(p, b);
   if (key >= L) return;
-  const int sees = first_row(key / KEYS * KEYS, L - p.T, p.Hq / p.Hkv) / ROWS * ROWS;
+  const int sees = first_row(key / kWeightsKeys * kWeightsKeys, L - p.T, p.Hq / p.Hkv) / kWeightsStage * kWeightsStage;
   const int64_t nbh = static_cast<int64_t>(p.B) * p.Hkv;
   float total = 0.f;
   for (int c = sees / p.chunk_rows; c < p.chunks; ++c) total += p.ws[(c * nbh + bh) * p.cap + key];
@@ -227,18 +218,18 @@ __global__ __launch_bounds__(256) void key_weights_join_kernel(KeyWeightsParams 
 
 namespace {
 
-template <typename T, int D, int KW, int RW, int NK>
+template <typename T, int D, int KW, int RW>
 hipError_t launch_weights(const KeyWeightsParams& p, hipStream_t s) {
-  using C = WeightsCfg<D, KW, RW, NK>;
+  using C = WeightsCfg<D, KW, RW>;
   const int ntiles = (p.cap + C::KEYS - 1) / C::KEYS;
   const int heads = p.B * p.Hkv;
   const int blocks = heads * ntiles * p.chunks;
-  hipLaunchKernelGGL((key_weights_kernel<T, D, KW, RW, NK>), folded_grid(blocks, C::NW * 64), dim3(C::NW * 64), 0, s,
+  hipLaunchKernelGGL((key_weights_kernel<T, D, KW, RW>), folded_grid(blocks, C::NW * 64), dim3(C::NW * 64), 0, s,
                      p, ntiles, blocks);
   if (p.chunks > 1) {
+    if (C::KEYS != kWeightsKeys || C::ROWS != kWeightsStage) return hipErrorInvalidValue;  // as the join counts them
     const int per = (p.cap + 255) / 256;
-    hipLaunchKernelGGL((key_weights_join_kernel<C::KEYS, C::ROWS>), folded_grid(heads * per, 256), dim3(256), 0, s, p,
-                       per, heads * per);
+    hipLaunchKernelGGL(key_weights_join_kernel, folded_grid(heads * per, 256), dim3(256), 0, s, p, per, heads * per);
   }
   return hipGetLastError();
 }
@@ -246,8 +237,9 @@ hipError_t launch_weights(const KeyWeightsParams& p, hipStream_t s) {
 template <typename T, int D>
 hipError_t launch_weights_t(const KeyWeightsParams& p, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(p.Hq / p.Hkv) * p.T;
-  if (rows <= 32) return launch_weights<T, D, 4, 1, 1>(p, s);
-  return launch_weights<T, D, 2, kWeightsStage / 32, kWeightsKeys / 64>(p, s);
+  constexpr int KW = kWeightsKeys / 32;
+  if (weights_one_wave(rows, weights_blocks(p.B, p.Hkv, p.cap))) return launch_weights<T, D, KW, 1>(p, s);
+  return launch_weights<T, D, KW, kWeightsStage / 32>(p, s);
 }
 
 template <typename T>

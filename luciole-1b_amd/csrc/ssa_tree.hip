@@ -13,13 +13,23 @@
 // matrix cores' columns:
 //   S^T = K Q^T (A = 32 keys from LDS, B = 32 rows of Q in registers)
 //   O^T += V^T P^T (A = V^T by LDS transpose reads, B = P^T from S^T)
-// so a lane pair (l, l + 32) holds one row.  Two forms:
-//   * up to 64 rows (tree_stream_kernel): the cache's stream is the bound; each
-//     wave streams its own tiles of 32 keys through a private LDS ring, for one
-//     or two groups of 32 rows at once, and the waves merge at the end;
-//   * more (tree_kernel): the transform (one log2 and one exp2 a pair) is
-//     the bound; QW groups of 32 rows by KW key waves share each stage of keys,
-//     and the key waves merge at the end.
+// so a lane pair (l, l + 32) holds one row.  A workgroup is QW groups of 32 rows by
+// KW key waves: each stage of keys goes to LDS once, by direct-to-LDS loads two
+// stages deep, for all groups; every wave takes its own tiles of 32 keys, and the
+// key waves of a group meet at the end.  What bounds it:
+//   * the stream of the cache where the rows are few: 16 x 16 heads x 4096 x 128
+//     in fp16, 64 nodes, takes 92 us, 5.6 TB/s of the rows that the sequences hold (the
+//     first form, each wave with tiles of its own and 32 rows, took 132, tiles that are not
+//     whole rows 106);
+//   * the transform where they are many: 73 VALU and 32 transcendental instructions for
+//     32 x 32 scores, 804 cycles of one SIMD, beside which the products (256 cycles at
+//     D = 64) are hidden: 1 x 32/8 x 65536 x 64, 64 nodes, has 46 to 49 us of
+//     transforms at the 2.1 GHz that the GPU holds then and takes 74, merge included;
+//   * a workgroup's start and end where both are few: 8 to 12 us, of which the load of
+//     the length, the first stage's latency, the exchange and the stores are 3 to 5
+//     each: 1 x 16 x 2048 x 128, 8 nodes, takes 14 us.
+// How many rows a workgroup has, and how many splits the keys, is in tree_plan().
+//
 // The keys are split over workgroups in ranges of one length for all sequences
 // (a ragged batch is then a number of equal pieces of work, and a sequence's
 // result does not depend on the others); partials (m, l, acc) meet in split
@@ -31,7 +41,10 @@
 // and the tile's maximum, a quarter of the vector work, are rare.
 //
 // The mask is packed to one bit per node when a workgroup's keys reach the
-// tree's rows; tiles before them do no mask work.
+// tree's rows; stages before them run in a loop of its own without any mask work.
+// Packing takes a workgroup 4000 cycles and the masked tiles as long again, in
+// the last split only; fetching the mask's bytes before the first stage's loads
+// put its registers into both loops and made 1 x 32/8 x 65536 x 64 80 us for 74.
 #include "ssa_cache_ops.hpp"
 #include "ssa_common.hpp"
 #include "ssa_launch.hpp"
@@ -316,8 +329,8 @@ struct RowOut {
 template <int D, int QW, int KW>
 struct TreeCfg {
   static constexpr int NW = QW * KW;
-  // tiles of a wave and stage: two where that leaves the stage at 64 KB (a longer
-  // first stage costs a short range of keys more than its barriers)
+  // tiles of a wave and stage: two where a stage's K and V then take 40 KB at
+  // most (a longer first stage costs a short range of keys more than its barriers)
   static constexpr int U = 2 * KW * 2 * RowTile<D>::BLOCK <= 40 * 1024 ? 2 : 1;
   static constexpr int BLOCKS = KW * U;
   static constexpr int KEYS = 32 * BLOCKS;
@@ -515,7 +528,10 @@ __global__ __launch_bounds__(QW* KW * 64) void tree_kernel(TreeParams p, int nun
 // The splits' partials of a row in split order: out = sum_s acc_s 2^(m_s - M) /
 // sum_s l_s 2^(m_s - M).  D / 4 threads a row, four columns each, and SW such
 // groups that take every SW-th split and meet in LDS; every load is independent
-// of the running state.
+// of the running state.  A launch and two dependent loads: 3.8 us for 128 rows of 8
+// splits, 5.9 for 2048 of 32 (17 MB).  SW = 4 pays from more than 8 splits on (32
+// splits of 128 rows x 64, the whole call: 14.7 us, SW = 1 16.2; 8 splits: 13.5 and
+// 12.6).
 template <typename T, int D, int SW>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p, int nrows) {
   typedef T v4 __attribute__((ext_vector_type(4)));
@@ -575,21 +591,22 @@ void launch_merge(const TreeParams& p, hipStream_t s) {
 template <typename T, int D>
 hipError_t launch_tree_t(const TreeParams& p, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(p.Hq / p.Hkv) * p.T;
-  const int per = tree_rows_per_block(rows);
-  const int nqb = static_cast<int>((rows + per - 1) / per);
-  const int units = static_cast<int>(tree_units(p.B, p.Hq, p.Hkv, p.T) * p.splits);
+  const int nqb = static_cast<int>((rows + p.rows - 1) / p.rows);
+  const int units = static_cast<int>(static_cast<int64_t>(p.B) * p.Hkv * nqb * p.splits);
   const auto go = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, folded_grid(units, threads), dim3(threads), 0, s, p, units, nqb);
   };
   constexpr int W = D == 128 ? 8 : 16;  // waves of a workgroup: 128 KB of LDS, 128 or 256 registers
-  if (per == 32)
+  if (p.rows == 32)
     go(tree_kernel<T, D, 1, W / 2>, W / 2 * 64);
-  else if (per == 64)
+  else if (p.rows == 64)
     go(tree_kernel<T, D, 2, W / 2>, W * 64);
-  else if (per == 128)
+  else if (p.rows == 128)
     go(tree_kernel<T, D, 4, W / 4>, W * 64);
-  else
+  else if (p.rows == 256)
     go(tree_kernel<T, D, 8, W / 8>, W * 64);
+  else
+    return hipErrorInvalidValue;
   if (p.splits > 8)
     launch_merge<T, D, 4>(p, s);
   else if (p.splits > 1)
