@@ -147,6 +147,34 @@ def test_tree_keeps_unseen_values_out(gpu, D, G, T, dtype):
     assert bool(out[:, :, rows][..., keep].isfinite().all())
 
 
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("G,splits", [(1, 0), (1, 2), (2, 0), (2, 2), (4, 0), (4, 2)])
+def test_tree_workgroups_of_more_rows(gpu, D, dtype, G, splits):
+    """61, 122 and 244 rows on workgroups of 64, 128 and 256: 256 (sequence, kv-head)
+    pairs, so that smaller ones would take more rounds of the GPU.  Empty rows,
+    empty sequences, and NaN and infinities where nothing looks."""
+    B, Hk, cap, T = 16, 16, 300, 61
+    _say(f"tree D={D} {dtype} G={G} splits={splits} wide workgroups")
+    lens = [300, 0, 1, 61, 60, 62, 299, 256, 257, 288, 317, 100, 150, 200, 250, 128]
+    k, v, g = _caches(gpu, B, Hk, cap, D, dtype, seed=G + D)
+    q = _randn((B, G * Hk, T, D), g, dtype, gpu)
+    mask = _random_tree(T, G, B)
+    mask[3, ::4] = False
+    unseen = [T - 1, T // 2]
+    mask[:, :, unseen] = False
+    clean, cm = _check_tree(gpu, q, k, v, lens, mask, splits=splits)
+    for i, L in enumerate(lens):
+        for j, value in zip(unseen, (math.nan, math.inf)):
+            if 0 <= min(L, cap) - T + j:
+                k[i, :, min(L, cap) - T + j] = value
+                v[i, :, min(L, cap) - T + j] = -value
+        k[i, :, L:] = math.inf
+        v[i, :, L:] = math.nan
+    out, m = _check_tree(gpu, q, k, v, lens, mask, splits=splits)
+    assert torch.equal(out, clean) and torch.equal(m, cm)
+
+
 def _check_seen(dev, q, k, v, lens, mask):
     from SSA import ssa_tree_attention
 
@@ -326,6 +354,19 @@ def test_weights_strides_and_sums(gpu):
     ssa_key_weights(qf, k, m, [L, L], w, 0.125, 1.5, 0.8)
     # 2 heads a group, 200 queries each, of probability 1; m comes from the forward's own fp32 sums
     assert torch.allclose(w.sum(-1), torch.full((2, 2), 2.0 * L, device=gpu), rtol=2.0 ** -12)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("B,Hq,Hk,cap,T,lens", [
+    (2, 4, 4, 1000, 65, [1000, 64]),        # 65 rows on few workgroups: two waves of rows
+    (2, 8, 2, 257, 100, [257, 30]),         # 400 rows
+    (16, 16, 16, 1024, 65, [1024, 1000, 65, 64, 1, 0, 129, 128] * 2),  # 2048 workgroups: one wave
+    (16, 32, 16, 1024, 300, [1024, 1000, 300, 299, 1, 0, 513, 512] * 2),  # ... of 600 rows: two
+])
+def test_weights_of_either_form(gpu, D, B, Hq, Hk, cap, T, lens):
+    _say(f"weights D={D} B={B} Hq={Hq} Hk={Hk} cap={cap} T={T}")
+    k, _, g = _caches(gpu, B, Hk, cap, D, BF16, seed=D + T)
+    _check_weights(gpu, _randn((B, Hq, T, D), g, BF16, gpu), k, lens)
 
 
 def test_weights_of_chunks_that_do_not_divide(gpu):
