@@ -89,8 +89,8 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* waves, int 
 // every step, less reads the weights again in every pass (whole calls: 8 x 8 x
 // 1024 x 64, E = 4 10.4 us, 16 15.0, 32 18.7; 16384 rows, E = 16 26.9, 4 30.1, 32
 // 31.5; 1 x 16 x 32768, E = 32 35, 16 40, 4 44; at 8192 rows E = 4 would be 7 %
-// faster than 16).  E = 64 needs more registers than 1024 threads have; the second
-// stretch in LDS takes 65536 rows from 63 to 55 us.  Rows that stay in any case are
+// faster than 16).  E = 64 was slower than 32; the
+// second stretch in LDS takes 65536 rows from 63 to 55 us.  Rows that stay in any case are
 // left out of the histograms, and 256 rows past the length at once: their lanes
 // would add to one bin, 78 us for 28 with 6451 such rows of 32972.
 template <int E, bool kFar = false>

@@ -15,9 +15,11 @@
 // split over workgroups in chunks, whose sums a second kernel adds up in their
 // order.
 //
-// With few rows the stream of K is the bound: 16 x 32/8 heads x 4096 x 64 with one
-// query takes 14.4 us (67 MB of K and 8.4 of weights, 5.2 TB/s), 4 x 16 x 8192 x 128
-// with 32 queries 23.4 (4.5 TB/s of K).  With many it is the transform, one log2
+// With few rows the stream of K is the bound: 16 x 32/8 heads x 4096 x 64, 2048 to
+// 4096 rows a sequence, with one query takes 14.9 us for 53.5 MB (K, the weights in and out;
+// 3.6 TB/s, a copy 4.8), 4 x 16 x 8192 x 128 with 32 queries 25.8 for 104 MB (4.0).
+// K goes straight to registers, 32 keys a wave and once, so the waves of a CU
+// (20 at D = 64) are what keeps loads on their way.  With many it is the transform, one log2
 // and one exp2 a pair, 768 cycles for 32 x 32 pairs on one SIMD, beside which the
 // product (256 at D = 64) is hidden: 1 x 32/8 x 4096 x 64 with 4096 queries takes
 // 103 us and 4 for the join, of 93 to 96 for the transforms alone at the 2.1 GHz
