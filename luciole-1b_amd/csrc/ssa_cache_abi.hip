@@ -68,10 +68,10 @@ bool rows_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t T) {
   return bh < (1ll << 30) && bh * T < (1ll << 30);
 }
 
-bool tree_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t cap, int32_t T, int32_t requested) {
+bool tree_ok(int32_t B, int32_t Hq, int32_t Hkv, int32_t cap, int32_t T, int32_t requested, ssa::TreePlan& plan) {
   if (!cache_ok(B, Hkv, cap) || !rows_ok(B, Hq, Hkv, T) || T > SSA_TREE_MAX_NODES || requested < 0) return false;
   // workgroups over all splits, and the merge's threads, stay below 2^30
-  const ssa::TreePlan plan = ssa::tree_plan(B, Hq, Hkv, cap, T, requested);
+  plan = ssa::tree_plan(B, Hq, Hkv, cap, T, requested);
   return plan.units * plan.splits < (1ll << 30);
 }
 
@@ -94,23 +94,24 @@ extern "C" {
 
 int32_t ssa_tree_num_splits(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t capacity, int32_t nodes,
                             int32_t requested) {
-  if (!tree_ok(batch, heads_q, heads_kv, capacity, nodes, requested)) return 0;
-  return ssa::tree_plan(batch, heads_q, heads_kv, capacity, nodes, requested).splits;
+  ssa::TreePlan plan;
+  return tree_ok(batch, heads_q, heads_kv, capacity, nodes, requested, plan) ? plan.splits : 0;
 }
 
 int64_t ssa_tree_workspace_bytes(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t capacity,
                                  int32_t head_dim, int32_t nodes, int32_t requested) {
-  if (!tree_ok(batch, heads_q, heads_kv, capacity, nodes, requested)) return 0;
+  ssa::TreePlan plan;
+  if (!tree_ok(batch, heads_q, heads_kv, capacity, nodes, requested, plan)) return 0;
   if (head_dim != 32 && head_dim != 64 && head_dim != 128) return 0;
-  const int64_t splits = ssa::tree_plan(batch, heads_q, heads_kv, capacity, nodes, requested).splits;
-  if (splits <= 1) return 0;
-  const int64_t recs = static_cast<int64_t>(batch) * heads_q * nodes * splits;
+  if (plan.splits <= 1) return 0;
+  const int64_t recs = static_cast<int64_t>(batch) * heads_q * nodes * plan.splits;
   return (tree_ml_floats(recs) + recs * head_dim) * 4;
 }
 
 int32_t ssa_tree_attention(const ssa_tree_args* a, void* stream) {
   if (a == nullptr) return SSA_ERR_NULL_POINTER;
-  if (!tree_ok(a->batch, a->heads_q, a->heads_kv, a->capacity, a->nodes, a->num_splits)) return SSA_ERR_SHAPE;
+  ssa::TreePlan plan;
+  if (!tree_ok(a->batch, a->heads_q, a->heads_kv, a->capacity, a->nodes, a->num_splits, plan)) return SSA_ERR_SHAPE;
   SSA_TRY(check_types(a->head_dim, a->dtype));
   SSA_TRY(check_tensor(a->q));
   SSA_TRY(check_tensor(a->k_cache));
@@ -120,8 +121,6 @@ int32_t ssa_tree_attention(const ssa_tree_args* a, void* stream) {
     return SSA_ERR_NULL_POINTER;
   if (a->mask_stride_b < 0) return SSA_ERR_ALIGNMENT;
   ssa::TreeParams p{};
-  const ssa::TreePlan plan =
-      ssa::tree_plan(a->batch, a->heads_q, a->heads_kv, a->capacity, a->nodes, a->num_splits);
   p.splits = plan.splits;
   p.split_keys = plan.split_keys;
   p.rows = plan.rows;

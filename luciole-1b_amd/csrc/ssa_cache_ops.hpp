@@ -98,8 +98,11 @@ inline TreePlan tree_plan(int B, int Hq, int Hkv, int cap, int T, int requested)
     if (most < 4) most = 4;
     if (requested > 0) most = requested;
     if (most > steps) most = steps;
-    for (int64_t s = requested > 0 ? most : 1; s <= most; ++s) {
-      const int64_t keys = (steps + s - 1) / s * kTreeStep, n = (cap + keys - 1) / keys;
+    int64_t per;  // steps of a split
+    // numbers of splits of one length of their own: the next is the least that shortens them
+    for (int64_t s = requested > 0 ? most : 1; s <= most; s = per > 1 ? (steps + per - 2) / (per - 1) : most + 1) {
+      per = (steps + s - 1) / s;
+      const int64_t keys = per * kTreeStep, n = (cap + keys - 1) / keys;
       const int64_t masked = T < keys ? T : keys;
       const int64_t cost = (units * n + kCUs - 1) / kCUs * (f.start + keys * f.key / 10) + (n > 1 ? kMerge : 0) +
                            3 * masked * f.rows / 10;
