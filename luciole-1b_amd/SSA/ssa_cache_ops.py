@@ -147,8 +147,8 @@ def ssa_tree_attention(q, k_cache, v_cache, cache_seqlens, tree_mask, softmax_sc
     ``return_m``).  A token that sees nothing gets ``out = 0``, ``m = -inf``; a
     sequence shorter than T holds the tree's last tokens only.  What a token does
     not see does not reach it, NaN and infinities included.  A sequence's results
-    do not depend on the others', and are bitwise reproducible for one
-    ``num_splits`` and capacity.
+    do not depend on the others', and are bitwise reproducible for one set of
+    sizes and ``num_splits``.
     """
     if q.is_cuda:
         r = _lib.native().tree(q, k_cache, v_cache, cache_seqlens, tree_mask, softmax_scale, ssa_n, ssa_b, num_splits,

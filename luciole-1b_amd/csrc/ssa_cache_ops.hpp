@@ -70,7 +70,7 @@ struct TreePlan {
 
 // The plan of least estimated time, ns:
 //   rounds of one workgroup a CU * (start and end + keys of a split * time of one)
-//   + the merge's launch, if any + the masked keys of the last split
+//   + the merge's launch, if any, and its splits + the masked keys of the last split
 // The constants were fitted to 2300 measured calls on caches read from HBM: 28
 // shapes (1 to 64 sequences, 8 to 8192 rows of a group, 1000 to 65536 keys) at all
 // head dims, in every form and with 1 to 64 splits.  The plans chosen take 2 %
@@ -80,6 +80,8 @@ struct TreePlan {
 // 16384 x 64, 1024 nodes: 106, 32 rows 116, 128 rows 138, 256 rows 207, whose last
 // split holds all masked keys), long caches of many rows to 256 (1 x 32/8 x 65536 x
 // 64, 64 nodes: 73.8, 128 rows 77.5; head dim 128: 120, 128 rows 128, 64 rows 141).
+// A split's share of the merge counts where one head has a long cache (1 x 16/1 x
+// 65536 x 64, 2 nodes: 128 splits 16.9 us, 256 19.7, 64 18.5).
 constexpr int kTreeStep = 256, kCUs = 256;
 inline TreePlan tree_plan(int B, int Hq, int Hkv, int cap, int T, int requested) {
   struct Form {
@@ -87,7 +89,7 @@ inline TreePlan tree_plan(int B, int Hq, int Hkv, int cap, int T, int requested)
     int64_t start, key;  // ns; tenths of ns
   };
   constexpr Form kForms[] = {{32, 7000, 80}, {64, 9000, 110}, {128, 12000, 195}, {256, 12000, 350}};
-  constexpr int64_t kMerge = 4500;
+  constexpr int64_t kMerge = 4500, kMergeSplit = 20;
   const int64_t rows = static_cast<int64_t>(Hq / Hkv) * T;
   const int64_t steps = (static_cast<int64_t>(cap) + kTreeStep - 1) / kTreeStep;
   TreePlan best{};
@@ -104,8 +106,8 @@ inline TreePlan tree_plan(int B, int Hq, int Hkv, int cap, int T, int requested)
       per = (steps + s - 1) / s;
       const int64_t keys = per * kTreeStep, n = (cap + keys - 1) / keys;
       const int64_t masked = T < keys ? T : keys;
-      const int64_t cost = (units * n + kCUs - 1) / kCUs * (f.start + keys * f.key / 10) + (n > 1 ? kMerge : 0) +
-                           3 * masked * f.rows / 10;
+      const int64_t cost = (units * n + kCUs - 1) / kCUs * (f.start + keys * f.key / 10) +
+                           (n > 1 ? kMerge + kMergeSplit * n : 0) + 3 * masked * f.rows / 10;
       if (cost < least) {
         least = cost;
         best = TreePlan{f.rows, units, static_cast<int>(keys), static_cast<int>(n)};
