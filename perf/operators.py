@@ -19,7 +19,6 @@ Kinds of case (KV caches are [B, Hkv, capacity, D], lengths int32 [B]):
 
 from __future__ import annotations
 
-import functools
 import math
 import random
 import sys
@@ -33,7 +32,6 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 SSA_N, SSA_B = 1.5, 0.8  # the framework's initial n and b
 
 
-@functools.lru_cache(maxsize=None)
 def _framework():
     root = str(Path(__file__).resolve().parent.parent / "luciole-1b_amd")
     if root not in sys.path:
