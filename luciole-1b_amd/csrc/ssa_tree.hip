@@ -5,8 +5,9 @@
 //   out_i = sum_j p_ij v_j,  p_i = softmax over visible j of n sign(s) ln(1 + b |s|),  s = scale q_i . k_j
 // in base 2: t = n sign(s) log2(1 + scale b |q.k|), p = 2^(t - m), with the
 // running maximum and sum of the online softmax in fp32 and p rounded to the
-// input type for the product with V (the rounding errors of the keys are
-// independent, and together stay below the output's own rounding).
+// input type for the product with V, the type that the matrix cores take at full
+// rate: half a step of each key's share, independent from key to key.  In fp16 the
+// step would grow for small p; kTreeLift keeps them off that.
 //
 // The G q-heads of a group and their T nodes are R = G T rows over one stream
 // of keys, row r = node * G + head.  As in the decode step the rows are the
@@ -35,10 +36,10 @@
 // result does not depend on the others); partials (m, l, acc) meet in split
 // order in tree_merge_kernel.
 //
-// The reference m of a row's exponents is its running maximum only loosely: it
-// starts at 0 where that suits the first scores and moves to the maximum when a
-// lane's sum of a tile passes a bound (kTreeSum), so that the rescaling of acc
-// and the tile's maximum, a quarter of the vector work, are rare.
+// The reference m of a row's exponents is its running maximum only loosely (and
+// kTreeLift below it): it starts at an exponent of 0 where that suits the first scores and
+// moves on when a lane's sum of a tile passes a bound (kTreeSum), so that the
+// rescaling of acc and the tile's maximum, a quarter of the vector work, are rare.
 //
 // The mask is packed to one bit per node when a workgroup's keys reach the
 // tree's rows; stages before them run in a loop of its own without any mask work.
@@ -56,9 +57,21 @@ namespace {
 
 constexpr int kMaxNodes = 1024;
 constexpr int kMaskWords = kMaxNodes / 32 + 1;  // words of a packed mask row, one of padding
-// A lane's sum of 16 p with the old maximum: below it no p overflows fp16, and
+// The reference of a row's exponents lies this far below its largest one.  p in
+// fp16 has its full bits down to 2^-14 only, and below 2^-25 p would be nothing in
+// the product with V but not in the sum l: with p up to 2^10 (or a lane's sum of
+// at least that) a key counts within 2^-25 of 2^10, 2^-35 of its row's sum.  Keys of
+// 2^-25.06 beside a few of 1 were lost before (their share of the result, all of it
+// where the few have values of 0).  bf16 has fp32's range.
+template <typename T>
+constexpr float kTreeLift = __is_same(T, __bf16) ? 0.f : 10.f;
+// A lane's sum of 16 p with the old reference: up to it no p overflows fp16, and
 // sums of 2^30 keys stay far from fp32's range.
-constexpr float kTreeSum = 16384.f;
+template <typename T>
+constexpr float kTreeSum = __is_same(T, __bf16) ? 16384.f : 65504.f;
+// ... and the least one of a row that has seen nothing yet: 2^kTreeLift
+template <typename T>
+constexpr float kTreeFirst = __is_same(T, __bf16) ? 1.f : 1024.f;
 
 __device__ __forceinline__ int clamped_length(const TreeParams& p, int b) {
   const int L = load_table_entry(p.seqlens, b);
@@ -223,10 +236,10 @@ __device__ __forceinline__ void tree_tile(f32x16 s, const RowTileV<D>& rv, uint3
   v8 pb[2];
   bool done = false;
   if constexpr (!MASKED) {
-    // a row that has seen nothing yet starts from 0: then its sum has to be
-    // large enough as well
+    // a row that has seen nothing yet starts from an exponent of 0: then its sum
+    // has to be large enough as well
     const bool fresh = st.m == -INFINITY;
-    const float ref = fresh ? 0.f : st.m;
+    const float ref = fresh ? -kTreeLift<T> : st.m;
     float sum = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -235,7 +248,7 @@ __device__ __forceinline__ void tree_tile(f32x16 s, const RowTileV<D>& rv, uint3
       sum += pv;
       pb[r >> 3][r & 7] = static_cast<T>(pv);
     }
-    done = __all(sum <= kTreeSum && (!fresh || sum >= 1.f));
+    done = __all(sum <= kTreeSum<T> && (!fresh || sum >= kTreeFirst<T>));
     if (done) {
       st.m = ref;
       st.l += sum;
@@ -257,7 +270,7 @@ __device__ __forceinline__ void tree_tile(f32x16 s, const RowTileV<D>& rv, uint3
     z = pair_max(z);
     const float top = NPOS ? z : -z;
     const float tmax = z == -INFINITY ? -INFINITY : n * copysignf(fast_log2(fmaf(c, fabsf(top), 1.f)), top);
-    const float mnew = fmaxf(st.m, tmax);
+    const float mnew = fmaxf(st.m, tmax - kTreeLift<T>);
     const float alpha = fast_exp2(mnew == -INFINITY ? 0.f : st.m - mnew);
     st.m = mnew;
 #pragma unroll
