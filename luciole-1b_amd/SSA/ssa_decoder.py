@@ -217,6 +217,8 @@ class SelfAttention(nn.Module):
 
     def forward(self, x, rot, cache: Optional[SSAKVCache] = None, tree_mask=None, window=None):
         """rot = (cos, sin, cos_h, sin_h) from ``SSADecoder.rotary``."""
+        if tree_mask is not None and cache is None:
+            raise ValueError("tree_mask: a drafted tree stands behind a cached prefix, and there is no cache")
         q, k, v = self._qkv(x, rot)
         if cache is None:
             ctx = self.core_attention(q, k, v)
@@ -425,10 +427,12 @@ class SSADecoder(nn.Module):
         ``caches`` (one per layer) the tokens are positions start_pos .. and
         their keys / values are appended to the caches.  ``positions`` [B, S]
         gives every token a position of its own instead, and with ``tree_mask``
-        ([S, S] or [B, S, S]) the tokens are a drafted tree behind the cached
-        prefix (``SSAAttention.forward_tree``).  ``window``: how many of a
+        ([S, S] or [B, S, S]; only with ``caches``) the tokens are a drafted tree
+        behind the cached prefix (``SSAAttention.forward_tree``).  ``window``: how many of a
         prompt's last tokens add to the weights of a cache that tracks them
         (None: all)."""
+        if tree_mask is not None and caches is None:
+            raise ValueError("tree_mask: a drafted tree stands behind a cached prefix, and there are no caches")
         S = input_ids.shape[1]
         x = self.embedding(input_ids.t())  # [S, B, h]
         if positions is None:
