@@ -66,8 +66,10 @@ class SSAKVCache:
                         if track_weights else None)
         self._drafted = None  # (q, m, scale, n, b) of the last drafted tree, for the weights of its accepted path
 
+    @torch.no_grad()
     def append(self, key: torch.Tensor, value: torch.Tensor) -> None:
-        """Append ``T`` new tokens per sequence: key / value ``[B, Hkv, T, D]``."""
+        """Append ``T`` new tokens per sequence: key / value ``[B, Hkv, T, D]``.
+        The cache holds their values: no gradient reaches them through it."""
         self._drafted = None
         B, _, T, _ = key.shape
         pos = self.seqlens.long().unsqueeze(1) + torch.arange(T, device=key.device).unsqueeze(0)
@@ -232,15 +234,16 @@ class SSAAttention(nn.Module):
                 cache.add_weights(q[:, :, -w:], m[:, :, -w:], self.softmax_scale, n, b)
         return out.permute(2, 0, 1, 3).reshape(query.shape[0], query.shape[1], -1)
 
+    @torch.no_grad()
     def forward_tree(self, query, key, value, cache: SSAKVCache, tree_mask):
-        """One step over a drafted tree of T tokens per sequence.  query [T, B, Hq,
-        D], key/value [T, B, Hkv, D] -> context [T, B, Hq * D]; keys and values are
-        appended to ``cache``, and token i attends the cached prefix and the
+        """One step over a drafted tree of T tokens per sequence, without gradients.
+        query [T, B, Hq, D], key/value [T, B, Hkv, D] -> context [T, B, Hq * D]; keys
+        and values are appended to ``cache``, and token i attends the cached prefix and the
         tokens that ``tree_mask`` ([T, T] or [B, T, T]) gives it.  Then
         ``cache.accept`` keeps the path that was right."""
         n, b = self.get_ssa_params()
         cache.append(key.permute(1, 2, 0, 3), value.permute(1, 2, 0, 3))
-        q = query.permute(1, 2, 0, 3)
+        q = query.detach().permute(1, 2, 0, 3)  # kept for accept, without the graph behind it
         track = cache.weights is not None
         ctx = ssa_tree_attention(q, cache.k, cache.v, cache.seqlens, tree_mask, self.softmax_scale, n, b,
                                  return_m=track)

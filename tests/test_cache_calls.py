@@ -26,3 +26,37 @@ def test_a_tree_needs_caches():
     x = torch.zeros(4, 2, 64)
     with pytest.raises(ValueError, match="cache"):
         layer.self_attention(x, model.rotary(torch.arange(4)), None, mask)
+
+
+def _module_on_host(monkeypatch):
+    """An SSAAttention whose tree attention is a stand-in that runs on the host."""
+    import SSA.ssa_attention as module
+
+    def attention(q, k_cache, v_cache, lens, mask, scale, n, b, num_splits=0, return_m=False):
+        out = q.detach().clone()
+        return (out, torch.zeros(q.shape[:3])) if return_m else out
+
+    monkeypatch.setattr(module, "ssa_tree_attention", attention)
+    monkeypatch.setattr(module, "check_tree_call", lambda *args: None, raising=False)
+    return module.SSAAttention(2, 1, 64)
+
+
+@pytest.mark.parametrize("track", [False, True])
+def test_appends_hang_no_graph_on_the_cache(monkeypatch, track):
+    """Keys and values that need gradients leave none in the cache's buffers, and a
+    tree's queries, kept for its accepted path, hold no graph alive."""
+    from SSA import SSAKVCache
+
+    mod = _module_on_host(monkeypatch)
+    cache = SSAKVCache(2, 1, 16, 64, torch.bfloat16, "cpu", track_weights=track)
+    make = lambda T, H: torch.ones(T, 2, H, 64, dtype=torch.bfloat16, requires_grad=True) * 2  # noqa: E731
+    k, v = make(3, 1), make(3, 1)
+    cache.append(k.permute(1, 2, 0, 3), v.permute(1, 2, 0, 3))
+    assert not cache.k.requires_grad and not cache.v.requires_grad and cache.seqlens.tolist() == [3, 3]
+    assert bool((cache.k[:, :, :3] == 2).all()) and bool((cache.v[:, :, 3:] == 0).all())
+    q = make(4, 2)
+    ctx = mod.forward_tree(q, make(4, 1), make(4, 1), cache, torch.ones(4, 4).tril())
+    assert not cache.k.requires_grad and not cache.v.requires_grad and not ctx.requires_grad
+    if track:
+        kept = cache._drafted[0]
+        assert not kept.requires_grad and (kept._base is None or kept._base.grad_fn is None)
