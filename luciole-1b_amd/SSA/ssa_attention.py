@@ -36,7 +36,7 @@ from typing import Optional
 import torch
 from torch import nn
 
-from .ssa_cache_ops import ssa_cache_accept, ssa_cache_evict, ssa_key_weights, ssa_tree_attention
+from .ssa_cache_ops import check_tree_call, ssa_cache_accept, ssa_cache_evict, ssa_key_weights, ssa_tree_attention
 from .ssa_flash_attention import ssa_flash_attention, ssa_flash_attention_varlen
 from .ssa_hip_kernel import ssa_decode_attention, ssa_flash_attn_forward
 
@@ -240,8 +240,13 @@ class SSAAttention(nn.Module):
         query [T, B, Hq, D], key/value [T, B, Hkv, D] -> context [T, B, Hq * D]; keys
         and values are appended to ``cache``, and token i attends the cached prefix and the
         tokens that ``tree_mask`` ([T, T] or [B, T, T]) gives it.  Then
-        ``cache.accept`` keeps the path that was right."""
+        ``cache.accept`` keeps the path that was right.  A call that is refused
+        leaves the cache as it was."""
         n, b = self.get_ssa_params()
+        if query.shape[0] > cache.capacity:
+            raise ValueError(f"a tree of {query.shape[0]} tokens in a cache of {cache.capacity} rows")
+        tree_mask = torch.as_tensor(tree_mask, device=query.device)
+        check_tree_call(query.permute(1, 2, 0, 3), cache.k, cache.v, tree_mask)  # before anything is appended
         cache.append(key.permute(1, 2, 0, 3), value.permute(1, 2, 0, 3))
         q = query.detach().permute(1, 2, 0, 3)  # kept for accept, without the graph behind it
         track = cache.weights is not None

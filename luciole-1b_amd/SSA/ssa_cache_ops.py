@@ -28,6 +28,11 @@ from .ssa_hip_kernel import (_DTYPES, _check_cache_layout, _current, _is_pow2, _
                              _t4)
 
 MAX_TREE_NODES = 1024
+HEAD_DIMS = (32, 64, 128)
+
+
+def _on_gpu(t) -> bool:
+    return t.is_cuda
 
 
 def _check_caches(k_cache, v_cache, names=("k_cache", "v_cache")):
@@ -37,12 +42,14 @@ def _check_caches(k_cache, v_cache, names=("k_cache", "v_cache")):
             raise ValueError(f"{name} must be [B, Hkv, capacity, D]")
         if t.dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"unsupported dtype {t.dtype}: the caches are bf16 or fp16")
-        if not t.is_cuda:
+        if not _on_gpu(t):
             raise ValueError(f"{name} must be on the GPU")
     if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or k_cache.device != v_cache.device:
         raise ValueError("k_cache and v_cache must share shape, dtype and device")
     D = k_cache.shape[3]
     assert _is_pow2(D), f"Head dim D={D} must be a power of two"
+    if D not in HEAD_DIMS:
+        raise ValueError(f"head dim {D}: the cache operators take {HEAD_DIMS}")
     for t, name in zip((k_cache, v_cache), names):
         _check_cache_layout(t, name)
     return k_cache.shape
@@ -132,6 +139,20 @@ def ssa_tree_num_splits(B: int, Hq: int, Hkv: int, capacity: int, nodes: int, nu
     return int(_lib.lib().ssa_tree_num_splits(B, Hq, Hkv, capacity, nodes, num_splits))
 
 
+def check_tree_call(q, k_cache, v_cache, tree_mask):
+    """Raises for the queries, caches and mask that ``ssa_tree_attention`` does not
+    take; (q as [B, Hq, T, D], whether it came as [B, Hq, D], the mask on q's device)."""
+    B = _check_caches(k_cache, v_cache)[0]
+    q4, squeeze = _check_queries(q, k_cache)
+    T = q4.shape[2]
+    if T > MAX_TREE_NODES:
+        raise ValueError(f"a tree has at most {MAX_TREE_NODES} tokens, got {T}")
+    mask = torch.as_tensor(tree_mask, device=q.device)
+    if tuple(mask.shape) not in ((T, T), (B, T, T)):
+        raise ValueError(f"tree_mask must be [{T}, {T}] or [{B}, {T}, {T}], got {tuple(mask.shape)}")
+    return q4, squeeze, mask
+
+
 def ssa_tree_attention(q, k_cache, v_cache, cache_seqlens, tree_mask, softmax_scale, ssa_n, ssa_b, num_splits=0,
                        return_m=False):
     """The tokens of a drafted tree attend the cache, in one pass over it.
@@ -156,14 +177,9 @@ def ssa_tree_attention(q, k_cache, v_cache, cache_seqlens, tree_mask, softmax_sc
         if r is not None:
             r = _native_result(r, "ssa_tree_attention")
             return r if return_m else r[0]
-    B, Hkv, cap, D = _check_caches(k_cache, v_cache)
-    q4, squeeze = _check_queries(q, k_cache)
-    Hq, T = q4.shape[1], q4.shape[2]
-    if T > MAX_TREE_NODES:
-        raise ValueError(f"a tree has at most {MAX_TREE_NODES} tokens, got {T}")
-    mask = torch.as_tensor(tree_mask, device=q.device)
-    if tuple(mask.shape) not in ((T, T), (B, T, T)):
-        raise ValueError(f"tree_mask must be [{T}, {T}] or [{B}, {T}, {T}], got {tuple(mask.shape)}")
+    q4, squeeze, mask = check_tree_call(q, k_cache, v_cache, tree_mask)
+    B, Hq, T, D = q4.shape
+    Hkv, cap = k_cache.shape[1:3]
     mask = (mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0).contiguous()
     lens = _lens(cache_seqlens, B, q.device)
     n32, b32 = _scalar(ssa_n, q.device), _scalar(ssa_b, q.device)

@@ -60,3 +60,35 @@ def test_appends_hang_no_graph_on_the_cache(monkeypatch, track):
     if track:
         kept = cache._drafted[0]
         assert not kept.requires_grad and (kept._base is None or kept._base.grad_fn is None)
+
+
+def test_a_refused_tree_leaves_the_cache(monkeypatch):
+    """forward_tree raises before anything is appended."""
+    from SSA import SSAAttention, SSAKVCache
+
+    mod = SSAAttention(2, 1, 64)
+    cache = SSAKVCache(2, 1, 16, 64, torch.bfloat16, "cpu")  # on the host: refused
+    make = lambda T, H: torch.ones(T, 2, H, 64, dtype=torch.bfloat16)  # noqa: E731
+    with pytest.raises(ValueError):
+        mod.forward_tree(make(4, 2), make(4, 1), make(4, 1), cache, torch.ones(4, 4).tril())
+    assert cache.seqlens.tolist() == [0, 0] and bool((cache.k == 0).all())
+
+
+@pytest.mark.parametrize("T,mask,dtype,D", [
+    (4, (4, 3), torch.bfloat16, 64), (4, (3, 4, 4), torch.bfloat16, 64), (1025, (1025, 1025), torch.bfloat16, 64),
+    (17, (17, 17), torch.bfloat16, 64), (4, (4, 4), torch.float32, 64), (4, (4, 4), torch.float16, 64),
+    (4, (4, 4), torch.bfloat16, 256)])
+def test_what_a_tree_call_refuses(monkeypatch, T, mask, dtype, D):
+    """The checks that forward_tree makes before it appends, on tensors that say they
+    are on the GPU."""
+    import SSA.ssa_cache_ops as ops
+    from SSA import SSAAttention, SSAKVCache
+
+    monkeypatch.setattr(ops, "_on_gpu", lambda t: True, raising=False)
+    mod = SSAAttention(2, 1, D)
+    cache = SSAKVCache(2, 1, 16, D, torch.bfloat16, "cpu")
+    make = lambda H: torch.ones(T, 2, H, D, dtype=dtype)  # noqa: E731
+    with pytest.raises(ValueError) as why:
+        mod.forward_tree(make(2), make(1), make(1), cache, torch.ones(mask))
+    assert "GPU" not in str(why.value)
+    assert cache.seqlens.tolist() == [0, 0] and bool((cache.k == 0).all())
