@@ -111,7 +111,7 @@ class SSAKVCache:
             raise ValueError(f"the last tree had {drafted[0].shape[2]} nodes, not {nodes}")
         path = torch.as_tensor(path, device=self.k.device)
         accepted = torch.as_tensor(accepted, device=self.k.device)
-        held = self.seqlens >= nodes
+        held = self.seqlens.clamp(max=self.capacity) >= nodes
         self.seqlens.copy_(ssa_cache_accept(self.k, self.v, self.seqlens, path, accepted, nodes))
         self._drafted = None
         if self.weights is None or drafted is None:
@@ -119,7 +119,7 @@ class SSAKVCache:
         q, m, scale, n, b = drafted
         # the path's queries at the end of the sequence, rows that were not accepted before them
         depth = path.shape[1]
-        count = torch.where(held, accepted.clamp(0, depth), torch.zeros_like(accepted)).long()
+        count = accepted.long().clamp(0, depth).masked_fill(~held, 0)
         step = torch.arange(depth, device=path.device)[None, :] - (depth - count)[:, None]
         node = path.long().clamp(0, nodes - 1).gather(1, step.clamp_min(0))
         at = node[:, None, :].expand(-1, q.shape[1], -1)

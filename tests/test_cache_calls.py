@@ -92,3 +92,47 @@ def test_what_a_tree_call_refuses(monkeypatch, T, mask, dtype, D):
         mod.forward_tree(make(2), make(1), make(1), cache, torch.ones(mask))
     assert "GPU" not in str(why.value)
     assert cache.seqlens.tolist() == [0, 0] and bool((cache.k == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64, torch.int16, torch.uint8, torch.bool])
+def test_accepted_counts_of_any_integer_type(monkeypatch, dtype):
+    """A tracking cache takes what ssa_cache_accept takes: with counts of 8 bits
+    it raised after the rows had moved, for 300 nodes do not fit them."""
+    import SSA.ssa_attention as module
+    from SSA import SSAKVCache
+
+    mod = _module_on_host(monkeypatch)
+    nodes, seen = 300, {}
+    cache = SSAKVCache(2, 1, 512, 64, torch.bfloat16, "cpu", track_weights=True)
+    make = lambda T, H: torch.ones(T, 2, H, 64, dtype=torch.bfloat16)  # noqa: E731
+    mod.forward_tree(make(nodes, 2), make(nodes, 1), make(nodes, 1), cache, torch.ones(nodes, nodes).tril())
+
+    def accept(k, v, lens, path, accepted, n):
+        return (lens - n + accepted.to(torch.int32).clamp(0, path.shape[1])).int()
+
+    def weights(q, k, m, lens, w, *rest):
+        seen.update(m=m, lens=lens.tolist())
+
+    monkeypatch.setattr(module, "ssa_cache_accept", accept)
+    monkeypatch.setattr(module, "ssa_key_weights", weights)
+    path = torch.arange(nodes).expand(2, nodes)
+    cache.accept(path, torch.tensor([1, 0]).to(dtype), nodes)
+    assert cache.seqlens.tolist() == [1, 0] and seen["lens"] == [1, 0]
+    # one query counts for the first sequence, none for the second
+    assert (seen["m"] > -torch.inf).sum((1, 2)).tolist() == [2, 0]
+
+
+def test_nothing_is_accepted_of_more_nodes_than_rows(monkeypatch):
+    """Lengths past the capacity hold as many rows as there are: of a tree of more
+    nodes than that nothing is accepted, and no weights are added."""
+    import SSA.ssa_attention as module
+    from SSA import SSAKVCache
+
+    cache = SSAKVCache(1, 1, 8, 64, torch.bfloat16, "cpu", track_weights=True)
+    cache.seqlens += 20
+    cache._drafted = (torch.zeros(1, 2, 12, 64), torch.zeros(1, 2, 12), 0.1, 1.5, 0.8)
+    seen = []
+    monkeypatch.setattr(module, "ssa_cache_accept", lambda k, v, lens, *rest: lens.clamp(max=8))
+    monkeypatch.setattr(module, "ssa_key_weights", lambda q, k, m, *rest: seen.append(m))
+    cache.accept(torch.arange(3)[None], torch.tensor([3]), 12)
+    assert cache.seqlens.tolist() == [8] and all(bool((m == -torch.inf).all()) for m in seen)
