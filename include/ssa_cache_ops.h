@@ -108,7 +108,8 @@ int32_t ssa_key_weights(const ssa_key_weights_args* args, void* stream);
  * length are left as they are.
  */
 typedef struct ssa_cache_evict_args {
-  ssa_tensor4 k_cache, v_cache; /* updated; no two elements at one address */
+  ssa_tensor4 k_cache, v_cache; /* updated; no two elements at one address,
+                                   in one of them or in both */
   const float* weights;         /* [B, Hkv, capacity] fp32, the last dimension contiguous */
   int64_t weights_stride_b, weights_stride_h;
   const int32_t* cache_seqlens;
@@ -133,7 +134,8 @@ int32_t ssa_cache_evict(const ssa_cache_evict_args* args, void* stream);
  * behind the new length that no accepted node moved to are left as they are.
  */
 typedef struct ssa_cache_accept_args {
-  ssa_tensor4 k_cache, v_cache; /* updated; no two elements at one address */
+  ssa_tensor4 k_cache, v_cache; /* updated; no two elements at one address,
+                                   in one of them or in both */
   const int32_t* cache_seqlens;
   const int32_t* path;          /* device, [B][depth] contiguous */
   const int32_t* accepted;      /* device, [B] */

@@ -30,20 +30,54 @@ int32_t check_tensor(const ssa_tensor4& t) {
   return SSA_OK;
 }
 
-// Every element of a [B, H, S, D] view at an address of its own: the strides in
-// ascending order each step over everything below them.
-bool disjoint(const ssa_tensor4& t, int32_t B, int32_t H, int32_t S, int32_t D) {
+// The dimensions of a [B, H, S, D] view that have more than one step, by ascending stride.
+struct Steps {
   struct Dim {
     int64_t stride, size;
-  } d[3] = {{t.stride_b, B}, {t.stride_h, H}, {t.stride_s, S}};
-  std::sort(d, d + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
-  __int128 extent = D;
-  for (const Dim& x : d) {
-    if (x.size <= 1) continue;
-    if (x.stride < extent) return false;
-    extent += static_cast<__int128>(x.stride) * (x.size - 1);
+  } d[3];
+  int n = 0;
+  Steps(const ssa_tensor4& t, int32_t B, int32_t H, int32_t S) {
+    for (const Dim& x : {Dim{t.stride_b, B}, Dim{t.stride_h, H}, Dim{t.stride_s, S}})
+      if (x.size > 1) d[n++] = x;
+    std::sort(d, d + n, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
   }
-  return true;
+  // elements from the first to the last, both counted
+  __int128 span(int32_t D) const {
+    __int128 e = D;
+    for (int i = 0; i < n; ++i) e += static_cast<__int128>(d[i].stride) * (d[i].size - 1);
+    return e;
+  }
+  // every element at an address of its own: each stride steps over everything below it
+  bool disjoint(int32_t D) const {
+    __int128 extent = D;
+    for (int i = 0; i < n; ++i) {
+      if (d[i].stride < extent) return false;
+      extent += static_cast<__int128>(d[i].stride) * (d[i].size - 1);
+    }
+    return true;
+  }
+  // Of a disjoint view and its copy `apart` elements on: some element at one address.
+  // What the steps below the i-th add up to is less than its stride, so only the
+  // two numbers of steps next to apart / stride come into question.
+  bool meets(__int128 apart, int32_t D, int i) const {
+    if (i < 0) return apart < D && apart > -D;
+    const __int128 s = d[i].stride, low = apart / s - (apart % s < 0 ? 1 : 0);
+    for (__int128 k = low; k <= low + 1; ++k)
+      if (k < d[i].size && k > -d[i].size && meets(apart - k * s, D, i - 1)) return true;
+    return false;
+  }
+};
+
+// Keys and values that are both written: no address twice, in either or in both.
+// Where one reaches between the other's rows (one buffer of both) they have one layout.
+bool disjoint_caches(const ssa_tensor4& k, const ssa_tensor4& v, int32_t B, int32_t H, int32_t S, int32_t D) {
+  const Steps ks(k, B, H, S), vs(v, B, H, S);
+  if (!ks.disjoint(D) || !vs.disjoint(D)) return false;
+  const __int128 ka = reinterpret_cast<uintptr_t>(k.ptr), va = reinterpret_cast<uintptr_t>(v.ptr);
+  if (ka + 2 * ks.span(D) <= va || va + 2 * vs.span(D) <= ka) return true;
+  if ((B > 1 && k.stride_b != v.stride_b) || (H > 1 && k.stride_h != v.stride_h) || (S > 1 && k.stride_s != v.stride_s))
+    return false;
+  return !ks.meets((va - ka) / 2, D, ks.n - 1);
 }
 
 int32_t check_types(int32_t D, int32_t dtype) {
@@ -168,7 +202,7 @@ int32_t ssa_key_weights(const ssa_key_weights_args* a, void* stream) {
     return SSA_ERR_NULL_POINTER;
   if (!aligned4(a->m) || !aligned4(a->weights)) return SSA_ERR_ALIGNMENT;
   // every weight is written: rows of capacity floats, none over another
-  if (!disjoint({nullptr, a->weights_stride_b, a->weights_stride_h, 0}, a->batch, a->heads_kv, 1, a->capacity))
+  if (!Steps({nullptr, a->weights_stride_b, a->weights_stride_h, 0}, a->batch, a->heads_kv, 1).disjoint(a->capacity))
     return SSA_ERR_ALIGNMENT;
   ssa::KeyWeightsParams p{};
   p.chunks = ssa::weights_chunks(a->batch, a->heads_q, a->heads_kv, a->capacity, a->queries);
@@ -209,9 +243,8 @@ int32_t ssa_cache_evict(const ssa_cache_evict_args* a, void* stream) {
     return SSA_ERR_NULL_POINTER;
   if (!aligned4(a->weights) || !aligned4(a->weights_out) || !aligned4(a->kept)) return SSA_ERR_ALIGNMENT;
   if (a->weights_stride_b < 0 || a->weights_stride_h < 0 || a->seqlens_out == a->cache_seqlens ||
-      a->weights_out == a->weights || a->k_cache.ptr == a->v_cache.ptr ||
-      !disjoint(a->k_cache, a->batch, a->heads_kv, a->capacity, a->head_dim) ||
-      !disjoint(a->v_cache, a->batch, a->heads_kv, a->capacity, a->head_dim))
+      a->weights_out == a->weights ||
+      !disjoint_caches(a->k_cache, a->v_cache, a->batch, a->heads_kv, a->capacity, a->head_dim))
     return SSA_ERR_ALIGNMENT;
   ssa::EvictParams p{};
   p.k = to_t4(a->k_cache);
@@ -243,9 +276,8 @@ int32_t ssa_cache_accept(const ssa_cache_accept_args* a, void* stream) {
   SSA_TRY(check_tensor(a->v_cache));
   if (a->cache_seqlens == nullptr || a->path == nullptr || a->accepted == nullptr || a->seqlens_out == nullptr)
     return SSA_ERR_NULL_POINTER;
-  if (a->seqlens_out == a->cache_seqlens || a->k_cache.ptr == a->v_cache.ptr ||
-      !disjoint(a->k_cache, a->batch, a->heads_kv, a->capacity, a->head_dim) ||
-      !disjoint(a->v_cache, a->batch, a->heads_kv, a->capacity, a->head_dim))
+  if (a->seqlens_out == a->cache_seqlens ||
+      !disjoint_caches(a->k_cache, a->v_cache, a->batch, a->heads_kv, a->capacity, a->head_dim))
     return SSA_ERR_ALIGNMENT;
   ssa::AcceptParams p{};
   p.k = to_t4(a->k_cache);

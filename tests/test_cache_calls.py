@@ -136,3 +136,32 @@ def test_nothing_is_accepted_of_more_nodes_than_rows(monkeypatch):
     monkeypatch.setattr(module, "ssa_key_weights", lambda q, k, m, *rest: seen.append(m))
     cache.accept(torch.arange(3)[None], torch.tensor([3]), 12)
     assert cache.seqlens.tolist() == [8] and all(bool((m == -torch.inf).all()) for m in seen)
+
+
+CACHE_BYTES = 2 * 4 * 8 * 4096 * 64  # of the caches below
+
+
+@pytest.mark.parametrize("entry", ["ssa_cache_evict", "ssa_cache_accept"])
+@pytest.mark.parametrize("offset,strides", [
+    (16, None), (64, None), (128 * 100, None), (CACHE_BYTES - 128, None), (-128, None), (-CACHE_BYTES + 128, None),
+    (4096 * 128, None),                               # a head further
+    (64, (8 * 4096 * 128, 4096 * 128, 128)),          # rows that reach into each other's half
+    (192, (8 * 4096 * 128, 4096 * 128, 128)),
+    (2 * 64 * 4096, (8 * 4096 * 64, 64, 8 * 64)),     # another layout over the same bytes
+])
+def test_caches_that_overlap_are_refused(entry, offset, strides):
+    """Keys and values that share memory would be moved over each other."""
+    import ctypes
+
+    from SSA import _lib
+
+    base = 1 << 32
+    k = _lib.Tensor4(base, *((8 * 4096 * 64, 4096 * 64, 64) if strides is None or strides[2] == 512 else strides))
+    v = _lib.Tensor4(base + offset, *(strides or (8 * 4096 * 64, 4096 * 64, 64)))
+    far = 1 << 20
+    if entry == "ssa_cache_evict":
+        args = _lib.CacheEvictArgs(k, v, far, 8 * 4096, 4096, far, far + 64, far + 4096, far, 4, 8, 4096, 64,
+                                   _lib.SSA_DTYPE_BF16, 1024, 4, 64)
+    else:
+        args = _lib.CacheAcceptArgs(k, v, far, far, far, far + 64, 4, 8, 4096, 64, _lib.SSA_DTYPE_BF16, 16, 5)
+    assert getattr(_lib.lib(), entry)(ctypes.byref(args), None) == _lib.SSA_ERR_ALIGNMENT

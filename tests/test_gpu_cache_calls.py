@@ -45,3 +45,45 @@ def test_refused_trees_leave_the_cache(gpu):
     cache.seqlens -= 5
     got = mod.forward_tree(q.requires_grad_(), k.requires_grad_(), v, cache, torch.ones(5, 5, device=gpu).tril())
     assert torch.equal(got, want) and not got.requires_grad and not cache.k.requires_grad
+
+
+@pytest.mark.parametrize("layout", ["row", "token", "head", "slots"])
+def test_one_buffer_of_keys_and_values(gpu, layout):
+    """Keys and values side by side in one buffer share no element and are moved as
+    two buffers are; views that share some are refused and nothing moves."""
+    from SSA import ssa_cache_accept, ssa_cache_evict
+
+    _say(f"one buffer, by {layout}")
+    B, H, cap, D = 3, 2, 200, 64
+    g = torch.Generator().manual_seed(2)
+    make = lambda *shape: torch.randn(*shape, generator=g).to(BF16).to(gpu)  # noqa: E731
+    if layout == "row":
+        room = make(B, H, cap, 2 * D)
+        k, v, wrong = room[..., :D], room[..., D:], room[..., D // 2:D // 2 + D]
+    elif layout == "token":
+        room = make(B, cap, 2, H, D)
+        k, v, wrong = room[:, :, 0].transpose(1, 2), room[:, :, 1].transpose(1, 2), room[:, :, :, 0].transpose(1, 2)
+    elif layout == "head":
+        room = make(B, H, 2 * cap, D)
+        k, v, wrong = room[:, :, :cap], room[:, :, cap:], room[:, :, 5:cap + 5]
+    else:  # keys in slots 0, 2, 4 and values in 3, 5, 7
+        room = make(8, H, cap, D)
+        k, v, wrong = room[0:6:2], room[3:8:2], room[2:8:2]
+    kc, vc = k.clone(), v.clone()
+    lens = torch.tensor([200, 150, 40], dtype=torch.int32, device=gpu)
+    w = torch.rand(B, H, cap, generator=g).to(gpu)
+    path = torch.tensor([[1, 4, 9], [0, 2, 3], [5, 6, 7]], dtype=torch.int32, device=gpu)
+    count = torch.tensor([3, 2, 1], dtype=torch.int32, device=gpu)
+    before = room.clone()
+    for a, b in ((k, wrong), (wrong, k)):
+        with pytest.raises(ValueError):
+            ssa_cache_accept(a, b, lens, path, count, 10)
+        with pytest.raises(ValueError):
+            ssa_cache_evict(a, b, lens, w, 60)
+    torch.cuda.synchronize()
+    assert torch.equal(room, before)
+    one, two = ssa_cache_accept(k, v, lens, path, count, 10), ssa_cache_accept(kc, vc, lens, path, count, 10)
+    assert torch.equal(one, two) and torch.equal(k, kc) and torch.equal(v, vc)
+    one, two = ssa_cache_evict(k, v, lens, w, 60, 2, 8), ssa_cache_evict(kc, vc, lens, w, 60, 2, 8)
+    assert all(torch.equal(x, y) for x, y in zip(one, two)) and torch.equal(k, kc) and torch.equal(v, vc)
+    ssa_cache_evict(v, k, lens, w, 60)  # either of them first
