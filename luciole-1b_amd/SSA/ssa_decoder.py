@@ -540,18 +540,12 @@ class SSADecoder(nn.Module):
                              tree_mask=mask.to(dev)).argmax(-1).t().tolist()
                 paths, counts = [], []
                 for i, seq in enumerate(text):
-                    path = [0]
                     if len(seq) >= end:  # done: nothing stays
-                        paths.append(path)
+                        paths.append([0])
                         counts.append(0)
                         continue
-                    while True:
-                        seq.append(picks[i][path[-1]])
-                        step = [c for c in range(path[-1] + 1, 1 + len(drafted[i]))
-                                if parents[i][c] == path[-1] and nodes[i][c] == seq[-1]]
-                        if not step or len(seq) >= end:
-                            break
-                        path.append(step[0])
+                    path = longest_path(nodes[i], parents[i], picks[i], end - len(seq), len(drafted[i]))
+                    seq.extend(picks[i][c] for c in path)
                     paths.append(path)
                     counts.append(len(path))
                 most = max(map(len, paths))
@@ -581,6 +575,22 @@ def drafted_tree(texts, drafted, above, max_nodes: int, vocab: int):
     nodes = [[seq[-1], *d] + [0] * (T - 1 - len(d)) for seq, d in zip(texts, drafted)]
     parents = [[-1, *(q + 1 for q in a)] + [0] * (T - 1 - len(a)) for a in above]
     return nodes, parents, tree_mask_from_parents(parents)  # refuses a parent that is not before its child
+
+
+def longest_path(tokens, parents, picks, most: int, drafted: Optional[int] = None):
+    """The longest path from node 0 (the first of equally long ones, at most ``most``
+    nodes) on which every node holds the token that the model picked at its parent;
+    ``drafted``: how many of the nodes behind node 0 are drafted tokens (None: all)."""
+    last = len(tokens) - 1 if drafted is None else drafted
+    reach, then = [1] * (last + 1), [0] * (last + 1)  # nodes from here on; the next of them
+    for c in range(last, 0, -1):  # every child is behind its parent
+        up = parents[c]
+        if tokens[c] == picks[up] and reach[c] + 1 >= reach[up]:
+            reach[up], then[up] = reach[c] + 1, c
+    path = [0]
+    while then[path[-1]] and len(path) < most:
+        path.append(then[path[-1]])
+    return path
 
 
 def lookup_draft(ngram: int = 2, length: int = 8):

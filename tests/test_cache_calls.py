@@ -165,3 +165,24 @@ def test_caches_that_overlap_are_refused(entry, offset, strides):
     else:
         args = _lib.CacheAcceptArgs(k, v, far, far, far, far + 64, 4, 8, 4096, 64, _lib.SSA_DTYPE_BF16, 16, 5)
     assert getattr(_lib.lib(), entry)(ctypes.byref(args), None) == _lib.SSA_ERR_ALIGNMENT
+
+
+def test_the_longest_drafted_path_is_kept():
+    """Of siblings with one token the one that leads furthest; a path ends where the
+    model's pick was not drafted, or after `most` tokens."""
+    from SSA.ssa_decoder import longest_path
+
+    #        0
+    #     1     2     3      nodes 1 and 3 hold the token that the model picks
+    #           4     5 - 6
+    tokens, parents = [9, 7, 8, 7, 5, 4, 3], [-1, 0, 0, 0, 2, 3, 5]
+    picks = [7, 4, 5, 4, 1, 3, 2]
+    assert longest_path(tokens, parents, picks, 10) == [0, 3, 5, 6]
+    assert longest_path(tokens, parents, picks, 3) == [0, 3, 5]
+    assert longest_path(tokens, parents, picks, 1) == [0]
+    assert longest_path(tokens, parents, [8, 0, 5, 0, 1, 0, 0], 10) == [0, 2, 4]
+    assert longest_path(tokens, parents, [6] * 7, 10) == [0]
+    # of equally long ones the first
+    assert longest_path([9, 7, 7], [-1, 0, 0], [7, 1, 1], 10) == [0, 1]
+    # nodes that only fill a shorter draft up are no drafted tokens
+    assert longest_path([9, 0, 0], [-1, 0, 0], [0, 0, 0], 10, drafted=0) == [0]

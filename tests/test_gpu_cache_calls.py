@@ -87,3 +87,34 @@ def test_one_buffer_of_keys_and_values(gpu, layout):
     one, two = ssa_cache_evict(k, v, lens, w, 60, 2, 8), ssa_cache_evict(kc, vc, lens, w, 60, 2, 8)
     assert all(torch.equal(x, y) for x, y in zip(one, two)) and torch.equal(k, kc) and torch.equal(v, vc)
     ssa_cache_evict(v, k, lens, w, 60)  # either of them first
+
+
+def test_a_token_drafted_twice_does_not_end_the_path(gpu):
+    """Siblings with one token, the first of which nothing follows: the path goes on
+    through the other one, four drafted tokens a step."""
+    from SSA.ssa_decoder import SSADecoder, SSADecoderConfig
+
+    _say("a token drafted twice")
+    torch.manual_seed(0)
+    model = SSADecoder(SSADecoderConfig(num_layers=2, hidden_size=256, num_attention_heads=4, num_query_groups=2,
+                                        kv_channels=64, ffn_hidden_size=512, vocab_size=512, init_std=0.1))
+    model = model.to(gpu).eval()
+    ids = torch.randint(512, (2, 20), generator=torch.Generator().manual_seed(1)).to(gpu)
+    plain, _ = model.generate(ids, 24)
+
+    def twice(texts):
+        drafted, above = [], []
+        for seq, want in zip(texts, plain.tolist()):
+            tokens, parents, at = [], [], -1
+            for t in want[len(seq):len(seq) + 4] if seq == want[:len(seq)] else []:
+                tokens += [t, t]
+                parents += [at, at]
+                at = len(tokens) - 1
+            drafted.append(tokens)
+            above.append(parents)
+        return drafted, above
+
+    tokens, steps = model.generate_drafted(ids, 24, twice)
+    # five tokens a step where the tree's and the decode step's picks agree throughout
+    if torch.equal(tokens, plain):
+        assert steps <= 5
