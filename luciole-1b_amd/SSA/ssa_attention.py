@@ -220,11 +220,13 @@ class SSAAttention(nn.Module):
 
     @torch.no_grad()
     def forward_prompt(self, query, key, value, cache: SSAKVCache, window: Optional[int] = None):
-        """A prompt into an empty cache: query [S, B, Hq, D], key/value [S, B, Hkv, D]
-        -> context [S, B, Hq * D] of the dense causal forward, without
+        """A prompt into an empty cache of at least its length: query [S, B, Hq, D],
+        key/value [S, B, Hkv, D] -> context [S, B, Hq * D] of the dense causal forward, without
         gradients; keys and values go to ``cache``, and a tracking cache gains
         the attention that the last ``window`` tokens (None: all) paid."""
         n, b = self.get_ssa_params()
+        if query.shape[0] > cache.capacity:
+            raise ValueError(f"a prompt of {query.shape[0]} tokens in a cache of {cache.capacity} rows")
         q, k, v = (t.permute(1, 2, 0, 3) for t in (query, key, value))
         out, m = ssa_flash_attn_forward(q, k, v, self.softmax_scale, n, b, True)
         cache.append(k, v)

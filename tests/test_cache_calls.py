@@ -186,3 +186,20 @@ def test_the_longest_drafted_path_is_kept():
     assert longest_path([9, 7, 7], [-1, 0, 0], [7, 1, 1], 10) == [0, 1]
     # nodes that only fill a shorter draft up are no drafted tokens
     assert longest_path([9, 0, 0], [-1, 0, 0], [0, 0, 0], 10, drafted=0) == [0]
+
+
+def test_a_prompt_longer_than_its_cache_is_refused(monkeypatch):
+    """Before anything is computed or appended; one that fills the cache is taken."""
+    import SSA.ssa_attention as module
+    from SSA import SSAKVCache
+
+    monkeypatch.setattr(module, "ssa_flash_attn_forward",
+                        lambda q, k, v, *rest: (torch.zeros_like(q), torch.zeros(q.shape[:3])))
+    mod = module.SSAAttention(2, 1, 64)
+    cache = SSAKVCache(1, 1, 8, 64, torch.bfloat16, "cpu")
+    make = lambda T, H: torch.ones(T, 1, H, 64, dtype=torch.bfloat16)  # noqa: E731
+    with pytest.raises(ValueError, match="rows"):
+        mod.forward_prompt(make(9, 2), make(9, 1), make(9, 1), cache)
+    assert cache.seqlens.tolist() == [0] and bool((cache.k == 0).all())
+    mod.forward_prompt(make(8, 2), make(8, 1), make(8, 1), cache)
+    assert cache.seqlens.tolist() == [8]
