@@ -36,7 +36,8 @@ from typing import Optional
 import torch
 from torch import nn
 
-from .ssa_cache_ops import check_tree_call, ssa_cache_accept, ssa_cache_evict, ssa_key_weights, ssa_tree_attention
+from .ssa_cache_ops import (HEAD_DIMS, check_tree_call, ssa_cache_accept, ssa_cache_evict, ssa_key_weights,
+                            ssa_tree_attention)
 from .ssa_flash_attention import ssa_flash_attention, ssa_flash_attention_varlen
 from .ssa_hip_kernel import ssa_decode_attention, ssa_flash_attn_forward
 
@@ -53,11 +54,14 @@ class SSAKVCache:
     With ``track_weights``, ``weights`` (fp32 ``[B, Hkv, capacity]``) holds the
     attention that the queries so far paid to every cached key (0 behind the
     sequence); ``SSAAttention`` keeps it up to date, and ``evict`` cuts the
-    cache by it.
+    cache by it (bf16 and fp16, head dims 32, 64 and 128).
     """
 
     def __init__(self, batch: int, heads_kv: int, capacity: int, head_dim: int, dtype=torch.bfloat16,
                  device="cuda", track_weights: bool = False):
+        if track_weights and (dtype not in (torch.bfloat16, torch.float16) or head_dim not in HEAD_DIMS):
+            raise ValueError(f"weights are tracked in caches of bf16 or fp16 with head dims {HEAD_DIMS}, not of "
+                             f"{dtype} with {head_dim}")
         self.k = torch.zeros(batch, heads_kv, capacity, head_dim, dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
         self.seqlens = torch.zeros(batch, dtype=torch.int32, device=device)

@@ -203,3 +203,19 @@ def test_a_prompt_longer_than_its_cache_is_refused(monkeypatch):
     assert cache.seqlens.tolist() == [0] and bool((cache.k == 0).all())
     mod.forward_prompt(make(8, 2), make(8, 1), make(8, 1), cache)
     assert cache.seqlens.tolist() == [8]
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.bfloat16, 256), (torch.float16, 16)])
+def test_a_cache_tracks_what_the_operators_take(dtype, D):
+    """A cache whose weights no operator can add to is refused when it is made, not
+    at its first step, with the step's rows already in it."""
+    from SSA import SSAKVCache
+    from SSA.ssa_decoder import SSADecoder, SSADecoderConfig
+
+    assert SSAKVCache(1, 1, 8, D, dtype, "cpu").weights is None
+    with pytest.raises(ValueError):
+        SSAKVCache(1, 1, 8, D, dtype, "cpu", track_weights=True)
+    model = SSADecoder(SSADecoderConfig(num_layers=1, hidden_size=D, num_attention_heads=1, num_query_groups=1,
+                                        kv_channels=D, ffn_hidden_size=64, vocab_size=64))
+    with pytest.raises(ValueError, match="weights"):
+        model.generate(torch.zeros(1, 4, dtype=torch.long), 2, dtype=dtype, keep=100)
