@@ -26,32 +26,11 @@
 // that the GPU holds then.  Two groups of 32 keys a wave, so that an operand read
 // from LDS serves two products, took as long there (106 and 107 us) and 1.1 to 1.4
 // times as long at D = 128, where their registers halve the waves of a SIMD.
-#include "ssa_cache_ops.hpp"
+#include "ssa_cache_plan.hpp"
 #include "ssa_common.hpp"
 #include "ssa_launch.hpp"
-#include "ssa_tile.hpp"
 
 namespace ssa {
-
-namespace {
-
-template <int D, int KW, int RW>
-struct WeightsCfg {
-  static constexpr int NW = KW * RW;
-  static constexpr int KEYS = 32 * KW;
-  static constexpr int ROWS = 32 * RW;              // rows of a stage
-  static constexpr int QB = ROWS * D * 2;           // bytes of its Q rows
-  static constexpr int PIECES = BlockLayout<D>::IPB;  // 1 KB pieces of a 32-row block
-};
-
-__device__ __forceinline__ int clamped_length(const KeyWeightsParams& p, int b) {
-  const int L = load_table_entry(p.seqlens, b);
-  return L < 0 ? 0 : (L > p.cap ? p.cap : L);
-}
-// The first row whose query stands at `key` or behind it.
-__device__ __forceinline__ int first_row(int key, int first, int G) { return key > first ? (key - first) * G : 0; }
-
-}  // namespace
 
 template <typename T, int D, int KW, int RW>
 __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsParams p, int ntiles, int nblocks) {
@@ -67,21 +46,9 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
 
   const int block = folded_block();
   if (block >= nblocks) return;
-  // all (sequence, head) pairs of a key tile together: the tiles of most rows come first
-  const int nbh = p.B * p.Hkv;
-  const int chunk = block / (nbh * ntiles);
-  const int tile = (block - chunk * nbh * ntiles) / nbh, bh = block % nbh;
-  const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
-  const int L = clamped_length(p, b);
-  const int key0 = tile * C::KEYS;
-  if (key0 >= L) return;
-  const int G = p.Hq / p.Hkv, first = L - p.T;  // first: position of query 0
-  // rows from the stage of the first query that sees key0 on; those of the chunk
-  const int64_t chunk0 = static_cast<int64_t>(chunk) * p.chunk_rows;
-  const int R = static_cast<int>(min(static_cast<int64_t>(G) * p.T, chunk0 + p.chunk_rows));
-  const int sees = first_row(key0, first, G) / C::ROWS * C::ROWS;
-  const int rstart = max(sees, static_cast<int>(chunk0));
-  if (rstart >= R) return;  // of the key's other chunks
+  const WeightsUnit u(p, block, ntiles, C::KEYS, C::ROWS);
+  if (u.behind() || u.unseen()) return;
+  const int b = u.b, hk = u.hk, L = u.L, key0 = u.key0, G = u.G, first = u.first, rstart = u.rstart, R = u.R;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -94,42 +61,21 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
   // rows of whole blocks that see every key of the wave
   const int rall = first_row(kbase + 31, first, G);
 
-  // the row of its block that this lane's loads fetch, as (query, head), moved
-  // on by one stage at a time
-  const LoadLane ll(lane, kw, p.q.ss);
-  int t, g;
-  {
-    const int r = rstart + 32 * rw + ll.r;
-    t = r / G;
-    g = r - t * G;
-  }
-  const int dt = C::ROWS / G, dg = C::ROWS - dt * G;
-  const char* qbase = static_cast<const char*>(p.q.ptr) + (b * p.q.sb + static_cast<int64_t>(hk) * G * p.q.sh) * 2;
+  WeightsRows<D, KW, RW> rows(p, u, lane, kw, rw);
+  const char* qbase = weights_queries(p, u);
   const float* mbase = p.m + (static_cast<int64_t>(b) * p.Hq + hk * G) * p.T;
   const uint32_t lds0 = lds_addr(qs);
   float mv = 0.f;
   int pv = -1;
   auto issue = [&](int i) {
-    const bool in = t < p.T;
-    const int tt = in ? t : p.T - 1, gg = in ? g : G - 1;
-    const char* src = qbase + (gg * p.q.sh + tt * p.q.ss) * 2 + ll.hoff;
-    const uint32_t dst = lds0 + (i & 1) * C::QB + rw * BlockLayout<D>::BLOCK;
-#pragma unroll
-    for (int cp = 0; cp < C::PIECES / KW; ++cp) dma_global16(dst + (kw + KW * cp) * 1024, src + (kw + KW * cp) * 32);
-    if (C::PIECES < KW) {
-      if (kw < C::PIECES) dma_global16(dst + kw * 1024, src + kw * 32);
-    }
+    const auto r = rows.row(p, u);
+    rows.load(p, r, qbase, i, lds0, kw, rw);
     if (kw == 0 && hh == 0) {
-      mv = mbase[static_cast<int64_t>(gg) * p.T + tt];
+      mv = mbase[static_cast<int64_t>(r.g) * p.T + r.t];
       // chunks end with a stage, so a row past R is past the last query
-      pv = in && mv != -INFINITY ? first + tt : -1;
+      pv = r.in && mv != -INFINITY ? first + r.t : -1;
     }
-    t += dt;
-    g += dg;
-    if (g >= G) {
-      g -= G;
-      ++t;
-    }
+    rows.next(u);
   };
   issue(0);
 
@@ -146,8 +92,8 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
   for (int i = 0; i < nst; ++i) {
     if (kw == 0) {
       if (hh == 0) {
-        ms[i & 1][32 * rw + ll.r] = mv;
-        ps[i & 1][32 * rw + ll.r] = pv;
+        ms[i & 1][32 * rw + rows.ll.r] = mv;
+        ps[i & 1][32 * rw + rows.ll.r] = pv;
       }
       const bool any = __any(hh == 0 && pv < 0);
       if (lane == 0) odd[i & 1][rw] = any;
@@ -191,7 +137,7 @@ __global__ __launch_bounds__(KW* RW * 64) void key_weights_kernel(KeyWeightsPara
   if (hh == 0) part[wave][l32] = both;
   __syncthreads();
   float* w = p.chunks == 1 ? p.w + b * p.w_sb + hk * p.w_sh
-                           : p.ws + (static_cast<int64_t>(chunk) * nbh + bh) * p.cap;
+                           : p.ws + weights_slot(p, u.chunk, u.bh, 0);
   for (int e = tid; e < C::KEYS; e += C::NW * 64) {
     const int at = key0 + e;
     if (at >= L) break;
@@ -209,12 +155,10 @@ __global__ __launch_bounds__(256) void key_weights_join_kernel(KeyWeightsParams 
   if (block >= nblocks) return;
   const int bh = block / blocks_per_head, key = (block - bh * blocks_per_head) * 256 + threadIdx.x;
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
-  const int L = clamped_length(p, b);
+  const int L = clamped_length(load_table_entry(p.seqlens, b), p.cap);
   if (key >= L) return;
-  const int sees = first_row(key / kWeightsKeys * kWeightsKeys, L - p.T, p.Hq / p.Hkv) / kWeightsStage * kWeightsStage;
-  const int64_t nbh = static_cast<int64_t>(p.B) * p.Hkv;
   float total = 0.f;
-  for (int c = sees / p.chunk_rows; c < p.chunks; ++c) total += p.ws[(c * nbh + bh) * p.cap + key];
+  for (int c = weights_first_chunk(p, L, key); c < p.chunks; ++c) total += p.ws[weights_slot(p, c, bh, key)];
   p.w[b * p.w_sb + hk * p.w_sh + key] += total;
 }
 

@@ -41,25 +41,26 @@ struct RowTile {
 template <int D, bool K>
 struct RowLoad {
   uint32_t voff;
-  __device__ __forceinline__ static int row(int lane) {
+  __host__ __device__ __forceinline__ static int row(int lane) {
     using R = RowTile<D>;
     const int s = lane / R::LPR;
     return K ? R::k_slot_row(s) : s;
   }
-  __device__ __forceinline__ static int chunk(int lane) {
+  __host__ __device__ __forceinline__ static int chunk(int lane) {
     using R = RowTile<D>;
     return (lane % R::LPR) ^ (4 * R::swz(lane / R::LPR));
   }
-  __device__ __forceinline__ RowLoad(int lane, int64_t ss)
+  __host__ __device__ __forceinline__ RowLoad(int lane, int64_t ss)
       : voff(static_cast<uint32_t>(row(lane) * ss * 2 + chunk(lane) * 16)) {}
 };
 
 // BLOCKS blocks of rows row0 .. of g to LDS byte address lds, piece j from wave
 // j % NW; rows at and past nrows repeat the last.  Whole tiles whose rows span
 // less than 2^31 bytes go through one descriptor with 32-bit offsets.
-template <int D, int BLOCKS, int NW, bool K>
-__device__ __forceinline__ void row_tile_load(const char* g, int64_t ss, int row0, int nrows, uint32_t lds, int wave,
-                                              int lane, const RowLoad<D, K>& rl) {
+template <int D, int BLOCKS, int NW, bool K, typename Mem = DeviceMem>
+__host__ __device__ __forceinline__ void row_tile_load(const char* g, int64_t ss, int row0, int nrows, uint32_t lds,
+                                                       int wave, int lane, const RowLoad<D, K>& rl,
+                                                       const Mem& mem = Mem()) {
   using R = RowTile<D>;
   constexpr int N = BLOCKS * R::PIECES, PER = (N + NW - 1) / NW;
   if (row0 + 32 * BLOCKS <= nrows && ss * 2 * 32 * BLOCKS < (1ll << 31)) {
@@ -70,8 +71,8 @@ __device__ __forceinline__ void row_tile_load(const char* g, int64_t ss, int row
       const int j = wave + NW * i;
       if (N % NW != 0 && j >= N) break;
       const int blk = j / R::PIECES, p = j % R::PIECES;
-      dma_buffer16(lds + blk * R::BLOCK + R::off(p), rs, rl.voff,
-                   (32 * blk + (K ? R::k_piece_row(p) : R::v_piece_row(p))) * ss2);
+      mem.load16(lds + blk * R::BLOCK + R::off(p), rs, rl.voff,
+                 (32 * blk + (K ? R::k_piece_row(p) : R::v_piece_row(p))) * ss2);
     }
   } else {
     const char* gc = g + RowLoad<D, K>::chunk(lane) * 16;
@@ -80,7 +81,7 @@ __device__ __forceinline__ void row_tile_load(const char* g, int64_t ss, int row
       const int blk = j / R::PIECES, p = j % R::PIECES;
       int row = row0 + 32 * blk + (K ? R::k_piece_row(p) : R::v_piece_row(p)) + RowLoad<D, K>::row(lane);
       row = row < nrows ? row : nrows - 1;
-      dma_global16(lds + blk * R::BLOCK + R::off(p), gc + row * ss * 2);
+      mem.load16_global(lds + blk * R::BLOCK + R::off(p), gc + row * ss * 2);
     }
   }
 }
@@ -90,7 +91,7 @@ template <int D>
 struct RowTileK {
   static constexpr int Q = D / 32;  // 64-byte quarters of a row
   uint32_t b[Q];
-  __device__ __forceinline__ RowTileK(int l32, int hh) {
+  __host__ __device__ __forceinline__ RowTileK(int l32, int hh) {
     using R = RowTile<D>;
     const int p = D == 128 ? l32 >> 2 : D == 64 ? l32 & 3 : (l32 >> 2) & 1;
     const int s = D == 128 ? l32 & 3 : D == 64 ? l32 >> 2 : (l32 & 3) + 4 * (l32 >> 3);
@@ -99,9 +100,12 @@ struct RowTileK {
       b[q] = static_cast<uint32_t>(R::off(p) + s * R::ROWB + (q ^ R::swz(s)) * 64 + hh * 16);
   }
   // at: byte address of a block
+  __host__ __device__ __forceinline__ uint32_t address(uint32_t at, int ds) const {
+    return b[ds >> 1] + at + (ds & 1) * 32;
+  }
   template <typename V>
   __device__ __forceinline__ V read(uint32_t at, int ds) const {
-    return *(const __attribute__((address_space(3))) V*)(uintptr_t)(b[ds >> 1] + at + (ds & 1) * 32);
+    return *(const __attribute__((address_space(3))) V*)(uintptr_t)address(at, ds);
   }
 };
 
@@ -111,7 +115,7 @@ template <int D>
 struct RowTileV {
   static constexpr int Q = D / 32;
   uint32_t b[Q];
-  __device__ __forceinline__ explicit RowTileV(int lane) {
+  __host__ __device__ __forceinline__ explicit RowTileV(int lane) {
     using R = RowTile<D>;
     const int g = lane >> 4, i = lane & 15, hh = lane >> 5;
     // (piece, slot) of row 4 hh + i / 4; the rest of the row is an immediate
@@ -121,13 +125,18 @@ struct RowTileV {
     for (int db = 0; db < Q; ++db)
       b[db] = static_cast<uint32_t>(R::off(p) + s * R::ROWB + (db ^ R::swz(s)) * 64 + (g & 1) * 32 + (i & 3) * 8);
   }
+  // the lane's 8 bytes: row 16 ks + 8 hi + 4 hh + i / 4, columns 32 db + 16 (g & 1) + 4 (i & 3)
+  // .., for lane i of the wave's 16 lanes g
+  __host__ __device__ __forceinline__ uint32_t address(uint32_t at, int ks, int hi, int db) const {
+    using R = RowTile<D>;
+    const int imm = D == 128 ? R::off(4 * ks + 2 * hi) : D == 64 ? R::off(2 * ks + hi) : R::off(ks) + hi * 8 * R::ROWB;
+    return b[db] + at + imm;
+  }
   template <typename V4>
   __device__ __forceinline__ V4 read(uint32_t at, int ks, int hi, int db) const {
-    using R = RowTile<D>;
     typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
-    const int imm = D == 128 ? R::off(4 * ks + 2 * hi) : D == 64 ? R::off(2 * ks + hi) : R::off(ks) + hi * 8 * R::ROWB;
     const bf16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-        (__attribute__((address_space(3))) bf16x4_t*)(uintptr_t)(b[db] + at + imm));
+        (__attribute__((address_space(3))) bf16x4_t*)(uintptr_t)address(at, ks, hi, db));
     return __builtin_bit_cast(V4, v);
   }
 };

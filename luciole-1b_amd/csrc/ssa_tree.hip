@@ -46,17 +46,14 @@
 // Packing takes a workgroup 4000 cycles and the masked tiles as long again, in
 // the last split only; fetching the mask's bytes before the first stage's loads
 // put its registers into both loops and made 1 x 32/8 x 65536 x 64 80 us for 74.
-#include "ssa_cache_ops.hpp"
+#include "ssa_cache_plan.hpp"
 #include "ssa_common.hpp"
 #include "ssa_launch.hpp"
-#include "ssa_row_tile.hpp"
 
 namespace ssa {
 
 namespace {
 
-constexpr int kMaxNodes = 1024;
-constexpr int kMaskWords = kMaxNodes / 32 + 1;  // words of a packed mask row, one of padding
 // The reference of a row's exponents lies this far below its largest one.  p in
 // fp16 has its full bits down to 2^-14 only, and below 2^-25 p would be nothing in
 // the product with V but not in the sum l: with p up to 2^10 (or a lane's sum of
@@ -72,51 +69,6 @@ constexpr float kTreeSum = __is_same(T, __bf16) ? 16384.f : 65504.f;
 // ... and the least one of a row that has seen nothing yet: 2^kTreeLift
 template <typename T>
 constexpr float kTreeFirst = __is_same(T, __bf16) ? 1.f : 1024.f;
-
-__device__ __forceinline__ int clamped_length(const TreeParams& p, int b) {
-  const int L = load_table_entry(p.seqlens, b);
-  return L < 0 ? 0 : (L > p.cap ? p.cap : L);
-}
-
-// What a workgroup works on.
-struct TreeUnit {
-  int b, hk, row0, nrows, split;  // rows row0 .. row0 + nrows - 1 of the group's R
-  int G, base, kbeg, kend, ntile;
-  const char* kg;
-  const char* vg;
-  float n, c;  // t = n sign(s) log2(1 + c |s|)
-  __device__ __forceinline__ TreeUnit(const TreeParams& p, int block, int per, int nqb) {
-    int u = block;
-    // the splits' first ranges of all sequences, then the second ones ...: the
-    // short last ranges come late
-    const int nbh = p.B * p.Hkv, whole = nbh * nqb;
-    split = u / whole;
-    u -= split * whole;
-    const int qb = u / nbh;
-    u -= qb * nbh;
-    b = u / p.Hkv;
-    hk = u - b * p.Hkv;
-    // the three scalars a workgroup waits for, on their way together
-    const int held = load_table_entry(p.seqlens, b);
-    n = __int_as_float(load_table_entry(reinterpret_cast<const int*>(p.n_ptr), 0));
-    c = p.scale * __int_as_float(load_table_entry(reinterpret_cast<const int*>(p.b_ptr), 0));
-    G = p.Hq / p.Hkv;
-    row0 = qb * per;
-    nrows = min(per, G * p.T - row0);
-    const int L = held < 0 ? 0 : (held > p.cap ? p.cap : held);
-    base = L - p.T;
-    const int64_t beg = static_cast<int64_t>(split) * p.split_keys;
-    kbeg = beg < L ? static_cast<int>(beg) : L;
-    kend = beg + p.split_keys < L ? static_cast<int>(beg + p.split_keys) : L;
-    ntile = (kend - kbeg + 31) / 32;
-    kg = static_cast<const char*>(p.k.ptr) + (b * p.k.sb + hk * p.k.sh) * 2;
-    vg = static_cast<const char*>(p.v.ptr) + (b * p.v.sb + hk * p.v.sh) * 2;
-  }
-  // a tile's keys that some rows may not see: the tree's
-  __device__ __forceinline__ bool masked(int key0) const { return key0 + 32 > base; }
-};
-
-__device__ __forceinline__ int mask_stride(int T) { return 2 * ((T + 63) / 64) + 1; }
 
 // Mask rows of the nodes of rows row0 .. row0 + nrows - 1, one bit a node, 64
 // nodes by one ballot; the word behind the last is 0.
@@ -324,38 +276,6 @@ __device__ __forceinline__ void add_not_finite(const TreeParams& p, const TreeUn
   }
 }
 
-// Element (row, d) of the result, or of the split's partial.
-struct RowOut {
-  int64_t rec;  // (global row) * splits + split
-  int64_t mrow;  // index into m [B, Hq, T]
-  int64_t off;   // element offset of the row in out
-  __device__ __forceinline__ RowOut(const TreeParams& p, const TreeUnit& u, int row) {
-    const int r = u.row0 + row, node = r / u.G, h = u.hk * u.G + r - node * u.G;
-    rec = ((static_cast<int64_t>(u.b) * p.Hkv + u.hk) * (u.G * p.T) + r) * p.splits + u.split;
-    mrow = (static_cast<int64_t>(u.b) * p.Hq + h) * p.T + node;
-    off = u.b * p.o.sb + h * p.o.sh + node * p.o.ss;
-  }
-};
-
-// Two stages of 32 KW U keys, a K tile and a V tile each; wave (qw, kw) takes
-// the stage's key tiles kw, kw + KW, ...
-template <int D, int QW, int KW>
-struct TreeCfg {
-  static constexpr int NW = QW * KW;
-  // tiles of a wave and stage: two where a stage's K and V then take 40 KB at
-  // most (a longer first stage costs a short range of keys more than its barriers)
-  static constexpr int U = 2 * KW * 2 * RowTile<D>::BLOCK <= 40 * 1024 ? 2 : 1;
-  static constexpr int BLOCKS = KW * U;
-  static constexpr int KEYS = 32 * BLOCKS;
-  static constexpr int TILE = BLOCKS * RowTile<D>::BLOCK;
-  // the key waves' exchange: each hands the others their shares of its acc
-  static constexpr int J = D / 8;                    // float4 of a lane's acc
-  static constexpr int JB = J > KW ? J / KW : 1;     // of a wave's share
-  static constexpr int MERGE = KW == 1 ? 0 : QW * J * (KW - 1) * 1024;
-  static constexpr int SMEM = 4 * TILE > MERGE ? 4 * TILE : MERGE;
-  static constexpr int WORDS = 32 * QW * kMaskWords > 128 * NW ? 32 * QW * kMaskWords : 128 * NW;
-};
-
 template <typename T, int D, bool NPOS, int QW, int KW>
 __device__ __forceinline__ void tree_body(const TreeParams& p, char* smem, uint32_t* words, int* bad,
                                           const TreeUnit& u) {
@@ -371,9 +291,7 @@ __device__ __forceinline__ void tree_body(const TreeParams& p, char* smem, uint3
   const uint32_t lds0 = lds_addr(smem);
   const int nst = (u.kend - u.kbeg + C::KEYS - 1) / C::KEYS;
   auto issue = [&](int i) {
-    const uint32_t dst = lds0 + (i & 1) * 2 * C::TILE;
-    row_tile_load<D, C::BLOCKS, NW, true>(u.kg, p.k.ss, u.kbeg + C::KEYS * i, u.kend, dst, wave, lane, lk);
-    row_tile_load<D, C::BLOCKS, NW, false>(u.vg, p.v.ss, u.kbeg + C::KEYS * i, u.kend, dst + C::TILE, wave, lane, lv);
+    tree_load_stage<D, QW, KW>(p, u, i, lds0, wave, lane, lk, lv);
   };
   if (nst > 0) issue(0);
   const float n = u.n, c = u.c;
@@ -556,8 +474,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p, int nrows
   const int G = p.Hq / p.Hkv, R = G * p.T;
   const int bh = row / R, r = row - bh * R, node = r / G;
   const int b = bh / p.Hkv, h = (bh - b * p.Hkv) * G + r - node * G;
-  const int64_t L = clamped_length(p, b);
-  const int ns = static_cast<int>((L + p.split_keys - 1) / p.split_keys);  // the sequence's own splits
+  const int ns = tree_own_splits(p, b);
   const int64_t rec0 = static_cast<int64_t>(row) * p.splits;
   const float* ml = p.ws_ml + 2 * rec0;
   // the row's lanes of a wave take a split each for the maximum and the sum
