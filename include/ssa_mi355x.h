@@ -49,7 +49,8 @@ enum {
   SSA_ERR_DTYPE = 4,          /* dtype not an SSA_DTYPE_* (decode: bf16 / fp16)   */
   SSA_ERR_ALIGNMENT = 5,      /* layout: base pointer not 16-byte aligned, a      */
                               /* stride negative or not a multiple of 8, or the   */
-                              /* row stride >= 2^24 elements                      */
+                              /* row stride >= 2^24 elements, or outputs that     */
+                              /* share memory (ssa_cache_ops.h)                   */
   SSA_ERR_LAUNCH = 6,         /* the HIP runtime rejected a kernel launch         */
   SSA_ERR_CU_SEQLENS = 7,     /* varlen: bad document table                       */
   SSA_ERR_SCRATCH = 8         /* ssa_bwd_noalloc: the problem's Delta + partials  */

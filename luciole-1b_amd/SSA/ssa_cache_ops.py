@@ -162,7 +162,8 @@ def ssa_tree_attention(q, k_cache, v_cache, cache_seqlens, tree_mask, softmax_sc
     ``cache_seqlens`` counts, token j of sequence b at row
     ``cache_seqlens[b] - T + j``.  Token i attends every row before the tree's
     and token j's where ``tree_mask[i, j]`` (bool ``[T, T]``, or ``[B, T, T]``
-    for a tree of its own per sequence; ``tree_mask_from_parents`` makes one).  A
+    for a tree of its own per sequence; ``tree_mask_from_parents`` makes one; in
+    another type, what is not 0 is seen, so an additive mask is none).  A
     lower triangular mask gives the causal attention of T consecutive tokens.
     Returns ``out`` shaped like ``q`` (and ``m [B, Hq, T]`` fp32 with
     ``return_m``).  A token that sees nothing gets ``out = 0``, ``m = -inf``; a

@@ -208,7 +208,7 @@ const char* ssa_status_string(int32_t status) {
     case SSA_ERR_DTYPE: return "unsupported dtype (supported: bf16, fp16, fp32; the decode step bf16, fp16)";
     case SSA_ERR_ALIGNMENT:
       return "unsupported tensor layout (base pointer 16-byte aligned, strides non-negative multiples of 8 "
-             "elements, row stride below 2^24 elements)";
+             "elements, row stride below 2^24 elements; what a call updates shares no memory)";
     case SSA_ERR_LAUNCH: return "HIP kernel launch failed";
     case SSA_ERR_CU_SEQLENS:
       return "invalid packed-sequence arguments (total_tokens, documents and max_seqlen must be > 0, "

@@ -15,7 +15,9 @@
 // What they take (bf16, the kernels alone): 8 x 8 heads x 4096 x 64 cut to 2048 rows,
 // selection 6 to 7 us and moves 10 to 11 (67 MB read and written, 6 to 6.5 TB/s);
 // 1 x 16 x 32768 x 128 cut to 4096, 24 and 16.  The selection is bound by the latency of its steps (three
-// passes over registers, each with two scans and five barriers) on one CU a head, the
+// passes over registers, each with two scans and five barriers) on one CU a head, and by
+// the scalar registers that its unrolled loops over the keys keep in vector registers (65
+// of the 16-key form, 169 of the 32-key one, 202 with a second stretch, none of the 4-key one), the
 // moves by their bytes where they fill the GPU and by the dependent chunks of a
 // slice where they do not.
 #include "ssa_cache_ops.hpp"

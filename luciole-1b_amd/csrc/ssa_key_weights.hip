@@ -16,13 +16,14 @@
 // order.
 //
 // With few rows the stream of K is the bound: 16 x 32/8 heads x 4096 x 64, 2048 to
-// 4096 rows a sequence, with one query takes 14.9 us for 53.5 MB (K, the weights in and out;
-// 3.6 TB/s, a copy 4.8), 4 x 16 x 8192 x 128 with 32 queries 25.8 for 104 MB (4.0).
+// 4096 rows a sequence, with one query takes 15.7 us for 53.5 MB (K, the weights in and out;
+// 3.4 TB/s, a copy 4.8), 4 x 16 x 8192 x 128 with 32 queries 23.5 for 104 MB (4.4).
 // K goes straight to registers, 32 keys a wave and once, so the waves of a CU
-// (20 at D = 64) are what keeps loads on their way.  With many it is the transform, one log2
-// and one exp2 a pair, 768 cycles for 32 x 32 pairs on one SIMD, beside which the
-// product (256 at D = 64) is hidden: 1 x 32/8 x 4096 x 64 with 4096 queries takes
-// 103 us and 4 for the join, of 93 to 96 for the transforms alone at the 2.1 GHz
+// (20 at D = 64) are what keeps loads on their way; a wave that has its scores has none
+// in flight.  With many it is the transform, one log2 and one exp2 a pair, 768 cycles
+// for 32 x 32 pairs on one SIMD, and the part of the product (128 cycles at D = 64) that is
+// not beside it, half by the counters: 1 x 32/8 x 4096 x 64 with 4096 queries takes
+// 108.5 us, 4 of them the join, and the transforms alone 93 to 96 at the 2.1 GHz
 // that the GPU holds then.  Two groups of 32 keys a wave, so that an operand read
 // from LDS serves two products, took as long there (106 and 107 us) and 1.1 to 1.4
 // times as long at D = 128, where their registers halve the waves of a SIMD.

@@ -6,8 +6,10 @@
 // in base 2: t = n sign(s) log2(1 + scale b |q.k|), p = 2^(t - m), with the
 // running maximum and sum of the online softmax in fp32 and p rounded to the
 // input type for the product with V, the type that the matrix cores take at full
-// rate: half a step of each key's share, independent from key to key.  In fp16 the
-// step would grow for small p; kTreeLift keeps them off that.
+// rate: half a step of each key's share, independent from key to key.  With 61
+// nodes over 1000 keys that makes the error of the output 0.0020 of its norm in
+// bf16, where its own rounding is 0.0017 (over 65536 keys 0.0017 with it, in fp16
+// 0.00025 and 0.00021).  In fp16 the step would grow for small p; kTreeLift keeps them off that.
 //
 // The G q-heads of a group and their T nodes are R = G T rows over one stream
 // of keys, row r = node * G + head.  As in the decode step the rows are the
@@ -19,16 +21,21 @@
 // stages deep, for all groups; every wave takes its own tiles of 32 keys, and the
 // key waves of a group meet at the end.  What bounds it:
 //   * the stream of the cache where the rows are few: 16 x 16 heads x 4096 x 128
-//     in fp16, 64 nodes, 2048 to 4096 rows a sequence, takes 92 us for 411 MB, 4.5 TB/s (the
+//     in fp16, 64 nodes, 2048 to 4096 rows a sequence, takes 93 us for 411 MB, 4.4 TB/s (the
 //     first form, each wave with tiles of its own and 32 rows, took 132, tiles that are not
 //     whole rows 106);
-//   * the transform where they are many: 73 VALU and 32 transcendental instructions for
-//     32 x 32 scores, 804 cycles of one SIMD, beside which the products (256 cycles at
-//     D = 64) are hidden: 1 x 32/8 x 65536 x 64, 64 nodes, has 46 to 49 us of
-//     transforms at the 2.1 GHz that the GPU holds then and takes 74, merge included;
+//   * the transform where they are many, and the products that stand alone: 73 VALU
+//     and 32 transcendental instructions for 32 x 32 scores, 804 cycles of one SIMD, and
+//     256 of products at D = 64, of which the counters have 56 % beside vector
+//     instructions.  Every stage's barrier lets the waves of a SIMD start their products
+//     together.  1 x 32/8 x 65536 x 64, 64 nodes, has 49 us of transforms and
+//     16 of products at the 2.1 GHz that the GPU holds then, and takes 73, merge
+//     included; 8 x 32/8 x 4096 x 64, 32 nodes, has 12 and 4 on its longest
+//     workgroups (2048 keys, 64 rows) and takes 29;
 //   * a workgroup's start and end where both are few: 8 to 12 us, of which the load of
 //     the length, the first stage's latency, the exchange and the stores are 3 to 5
-//     each: 1 x 16 x 2048 x 128, 8 nodes, takes 14 us.
+//     each: 1 x 16 x 2048 x 128, 8 nodes, takes 14 us.  At head dims 64 and 128
+//     LDS holds one workgroup a CU, so no other one fills that time.
 // How many rows a workgroup has, and how many splits the keys, is in tree_plan().
 //
 // The keys are split over workgroups in ranges of one length for all sequences
@@ -46,6 +53,9 @@
 // Packing takes a workgroup 4000 cycles and the masked tiles as long again, in
 // the last split only; fetching the mask's bytes before the first stage's loads
 // put its registers into both loops and made 1 x 32/8 x 65536 x 64 80 us for 74.
+//
+// The compiler keeps 5 (bf16) and 6 (fp16) registers of the 256-row form at D = 64 in scratch in
+// the body for n < 0 (8 bytes reloaded a stage), none in the one for n >= 0.
 #include "ssa_cache_plan.hpp"
 #include "ssa_common.hpp"
 #include "ssa_launch.hpp"
