@@ -115,10 +115,11 @@ class SSAKVCache:
             raise ValueError(f"the last tree had {drafted[0].shape[2]} nodes, not {nodes}")
         path = torch.as_tensor(path, device=self.k.device)
         accepted = torch.as_tensor(accepted, device=self.k.device)
-        held = self.seqlens.clamp(max=self.capacity) >= nodes
+        weighs = self.weights is not None and drafted is not None
+        held = self.seqlens.clamp(max=self.capacity) >= nodes if weighs else None
         self.seqlens.copy_(ssa_cache_accept(self.k, self.v, self.seqlens, path, accepted, nodes))
         self._drafted = None
-        if self.weights is None or drafted is None:
+        if not weighs:
             return
         q, m, scale, n, b = drafted
         # the path's queries at the end of the sequence, rows that were not accepted before them
