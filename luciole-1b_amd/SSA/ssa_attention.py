@@ -232,13 +232,15 @@ class SSAAttention(nn.Module):
         n, b = self.get_ssa_params()
         if query.shape[0] > cache.capacity:
             raise ValueError(f"a prompt of {query.shape[0]} tokens in a cache of {cache.capacity} rows")
+        w = query.shape[0] if window is None else min(window, query.shape[0])
+        weighs = cache.weights is not None and w > 0
+        if weighs and query.dtype != cache.k.dtype:
+            raise ValueError(f"queries of {query.dtype} for the weights of a cache of {cache.k.dtype}")
         q, k, v = (t.permute(1, 2, 0, 3) for t in (query, key, value))
         out, m = ssa_flash_attn_forward(q, k, v, self.softmax_scale, n, b, True)
         cache.append(k, v)
-        if cache.weights is not None:
-            w = q.shape[2] if window is None else min(window, q.shape[2])
-            if w > 0:
-                cache.add_weights(q[:, :, -w:], m[:, :, -w:], self.softmax_scale, n, b)
+        if weighs:
+            cache.add_weights(q[:, :, -w:], m[:, :, -w:], self.softmax_scale, n, b)
         return out.permute(2, 0, 1, 3).reshape(query.shape[0], query.shape[1], -1)
 
     @torch.no_grad()

@@ -219,3 +219,20 @@ def test_a_cache_tracks_what_the_operators_take(dtype, D):
                                         kv_channels=D, ffn_hidden_size=64, vocab_size=64))
     with pytest.raises(ValueError, match="weights"):
         model.generate(torch.zeros(1, 4, dtype=torch.long), 2, dtype=dtype, keep=100)
+
+
+def test_a_prompt_whose_attention_cannot_be_weighed_is_refused(monkeypatch):
+    """Queries of another type than a tracking cache's: before anything is appended."""
+    import SSA.ssa_attention as module
+    from SSA import SSAKVCache
+
+    monkeypatch.setattr(module, "ssa_flash_attn_forward",
+                        lambda q, k, v, *rest: (torch.zeros_like(q), torch.zeros(q.shape[:3])))
+    mod = module.SSAAttention(2, 1, 64)
+    make = lambda H: torch.ones(4, 1, H, 64, dtype=torch.float16)  # noqa: E731
+    cache = SSAKVCache(1, 1, 8, 64, torch.bfloat16, "cpu", track_weights=True)
+    with pytest.raises(ValueError):
+        mod.forward_prompt(make(2), make(1), make(1), cache)
+    assert cache.seqlens.tolist() == [0] and bool((cache.k == 0).all())
+    mod.forward_prompt(make(2), make(1), make(1), cache, window=0)  # nothing to weigh
+    assert cache.seqlens.tolist() == [4]
